@@ -1,0 +1,381 @@
+// Attention of trees of drafted tokens over the paged cache: each sequence brings n nodes (tokens proposed for the places behind
+// its `length` cached ones), whose keys and values lie in its pages at places length .. length + n - 1.  A node sees the cached
+// keys and the nodes above it (and itself), said by a row of bits:
+//     key place j <  length:      seen when j > position - window            (position = length + depth in the tree)
+//     key place length + j:       seen when bit j of the node's mask is set and position_j > position - window
+//     o = sum softmax(scale q . k) v over the keys seen, fp32; no key seen: zeros.
+//
+//   draft_masks_kernel        the masks and positions from the nodes' parents, once a step
+//   draft_attention_kernel    any type, head size and page size, fp32 FMAs
+//   draft_join_kernel         joins the shares of the keys where they were split
+//
+// The tensor-core kernel for bf16 heads of 64 and 128 is csrc/drafts_tc.cu.
+#include "common.cuh"
+
+using namespace mlb;
+
+MLB_DEFINE_LAST_ERROR()
+
+namespace {
+
+constexpr int MAX_NODES = 256;
+constexpr int MAX_WORDS = MAX_NODES / 32;
+
+// ------------------------------------------------------------------------------ masks
+// A thread a node, walking up; a parent is an earlier node of the sequence or -1, so a walk ends.
+__global__ void __launch_bounds__(MAX_NODES) draft_masks_kernel(const int* __restrict__ parents, const int* __restrict__ starts, const int* __restrict__ lengths,
+                                                                int words, int* __restrict__ masks, int* __restrict__ positions, int* __restrict__ places,
+                                                                int* error_flag) {
+    pdl_prologue();
+    __shared__ int s_parent[MAX_NODES];
+    __shared__ unsigned s_bits[MAX_NODES * (MAX_WORDS + 1)];
+    const int a = blockIdx.x, i = threadIdx.x;
+    const int start = starts[a], length = lengths[a];
+    int n = starts[a + 1] - start;
+    if (n < 0 || n > words * 32) {
+        if (i == 0 && error_flag) atomicExch(error_flag, 3);
+        n = 0;
+    }
+    if (i < n) {
+        int parent = parents[start + i];
+        if (parent < -1 || parent >= i) {
+            if (error_flag) atomicExch(error_flag, 3);
+            parent = -1;
+        }
+        s_parent[i] = parent;
+    }
+    __syncthreads();
+    if (i >= n) return;
+    unsigned* const bits = s_bits + i * (words | 1);           // an odd pitch: neighbouring threads in different banks
+    for (int w = 0; w < words; ++w) bits[w] = 0u;
+    int depth = -1;
+    for (int node = i; node >= 0; node = s_parent[node]) {
+        bits[node >> 5] |= 1u << (node & 31);
+        ++depth;
+    }
+    for (int w = 0; w < words; ++w) masks[(size_t)(start + i) * words + w] = (int)bits[w];
+    positions[start + i] = length + depth;
+    if (places) places[start + i] = length + i;
+}
+
+// ------------------------------------------------------------------------------ attention
+constexpr int THREADS = 128;
+constexpr int ROWS = 16;                       // (node, head) rows of one kv head a CTA works on; a warp has four
+constexpr int KEYS = 32;                       // keys a tile: a lane each
+
+struct DraftParams {
+    const void* q;           // [T, ldq]
+    const void* pages;       // [num_pages, 2, NKV, page_size, D]
+    void* out;               // [T, NH * D]
+    const int* starts;       // [A + 1]
+    const int* lengths;      // [A]
+    const int* positions;    // [T]
+    const int* masks;        // [T, words]
+    const int* table;        // [A, max_blocks]
+    int words, max_blocks, num_pages, page_size;
+    int heads, kv_heads, group, dim, window, row_tiles;
+    int share;               // keys of one share, a multiple of KEYS
+    int shares;
+    int tokens, max_nodes;
+    float scale;
+    float* part_out;         // [shares, T * NH, D]     unnormalised
+    float2* part_norm;       // [shares, T * NH]        maximum, sum
+    int* error_flag;
+};
+
+// the first key that any node of a sequence may see
+__device__ __forceinline__ int first_key(int length, int window) { return window > 0 ? max(0, length - window + 1) : 0; }
+
+// PIECES: rows of the cache and of q are read in pieces of four elements.  COLS columns and RPT rows a thread in the second product.
+template <typename T, int DMAX, bool PIECES>
+__global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p) {
+    pdl_prologue();
+    constexpr int COLS = DMAX > 128 ? 2 : 1;
+    constexpr int RPT = DMAX >= 128 ? ROWS : DMAX / 8;         // 32: 4, 64: 8
+    constexpr int PITCH = DMAX + 4;
+    extern __shared__ float smem[];
+    float* const q_s = smem;                                   // [ROWS][DMAX]
+    float* const k_s = q_s + ROWS * DMAX;                      // [KEYS][PITCH]
+    float* const v_s = k_s + KEYS * PITCH;                     // [KEYS][DMAX]
+    __shared__ __align__(16) float p_s[ROWS][KEYS];
+    __shared__ float alpha_s[ROWS], sum_s[ROWS], max_s[ROWS];
+    __shared__ unsigned mask_s[ROWS][MAX_WORDS];
+    __shared__ int pos_s[ROWS], key_pos_s[KEYS];
+    __shared__ long long key_at[KEYS];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int share = blockIdx.x, seq = blockIdx.z;
+    const int kvh = blockIdx.y / p.row_tiles, row0 = (blockIdx.y % p.row_tiles) * ROWS;
+    const int start = p.starts[seq], n = p.starts[seq + 1] - start, length = p.lengths[seq];
+    const int G = p.group, D = p.dim;
+    const int rows = min(ROWS, n * G - row0);
+    if (rows <= 0) return;
+    if (n > p.max_nodes && tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);      // the grid has no rows for the last of them
+    // The shares begin at the first key that a row may see (positions are at least `length`); the last one takes what is left, so that a
+    // sequence longer than the caller said costs time and nothing else.
+    const int lo = first_key(length, p.window), total = length + n;
+    const int key_begin = lo / KEYS * KEYS + share * p.share;
+    const int key_end = share == p.shares - 1 ? total : min(total, key_begin + p.share);
+    if (share > 0 && key_begin >= total) return;
+
+    for (int e = tid; e < ROWS * DMAX; e += THREADS) {
+        const int r = e / DMAX, c = e % DMAX;
+        float v = 0.0f;
+        if (r < rows && c < D) {
+            const int row = row0 + r;
+            v = to_f32(((const T*)p.q)[(size_t)(start + row / G) * p.heads * D + (size_t)(kvh * G + row % G) * D + c]);
+        }
+        q_s[e] = v;
+    }
+    for (int e = tid; e < ROWS * p.words; e += THREADS) {
+        const int r = e / p.words, w = e % p.words;
+        mask_s[r][w] = r < rows ? (unsigned)p.masks[(size_t)(start + (row0 + r) / G) * p.words + w] : 0u;
+    }
+    if (tid < ROWS) pos_s[tid] = tid < rows ? p.positions[start + (row0 + tid) / G] : 0;
+
+    float acc[RPT][COLS];
+#pragma unroll
+    for (int r = 0; r < RPT; ++r)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[r][c] = 0.0f;
+    // second product: this thread's first row and column
+    const int my_row = DMAX >= 128 ? 0 : (tid / DMAX) * RPT, my_col = DMAX >= 128 ? tid : tid % DMAX;
+    float m[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
+    const size_t plane = (size_t)p.page_size * D, page_stride = 2 * plane * p.kv_heads, v_offset = plane * p.kv_heads;
+    const int* const table = p.table + (size_t)seq * p.max_blocks;
+
+    for (int base = key_begin; base < key_end; base += KEYS) {
+        __syncthreads();                                       // the last tile's values were read
+        if (tid < KEYS) {
+            const int key = base + tid;
+            long long at = -1;
+            int where = -1;
+            if (key >= lo && key < key_end) {
+                const int block = key / p.page_size;
+                const int page = block < p.max_blocks ? table[block] : -1;
+                if (page < 0 || page >= p.num_pages) {
+                    if (p.error_flag) atomicExch(p.error_flag, 2);
+                } else {
+                    at = (long long)((size_t)page * page_stride + (size_t)kvh * plane + (size_t)(key % p.page_size) * D);
+                    where = key < length ? key : p.positions[start + key - length];
+                }
+            }
+            key_at[tid] = at;
+            key_pos_s[tid] = where;
+        }
+        __syncthreads();
+        bool odd = false;                                      // a value that is not finite: it may not meet the zero weight of a row that does not see it
+        if (PIECES) {
+            constexpr int P = DMAX / 4;
+            for (int e = tid; e < KEYS * P; e += THREADS) {
+                const int key = e / P, c = (e % P) * 4;
+                const long long at = key_at[key];
+                float4 k4 = make_float4(0, 0, 0, 0), v4 = k4;
+                if (at >= 0 && c < D) {
+                    const T* const k = (const T*)p.pages + at + c;
+                    const T* const v = k + v_offset;
+                    if constexpr (sizeof(T) == 4) {
+                        k4 = *reinterpret_cast<const float4*>(k);
+                        v4 = *reinterpret_cast<const float4*>(v);
+                    } else {
+                        const uint2 a = *reinterpret_cast<const uint2*>(k), b = *reinterpret_cast<const uint2*>(v);
+                        k4 = make_float4(__uint_as_float(a.x << 16), __uint_as_float(a.x & 0xffff0000u), __uint_as_float(a.y << 16), __uint_as_float(a.y & 0xffff0000u));
+                        v4 = make_float4(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u));
+                    }
+                }
+                *reinterpret_cast<float4*>(k_s + key * PITCH + c) = k4;
+                *reinterpret_cast<float4*>(v_s + key * DMAX + c) = v4;
+                odd |= !(fabsf(v4.x) < INFINITY && fabsf(v4.y) < INFINITY && fabsf(v4.z) < INFINITY && fabsf(v4.w) < INFINITY);
+            }
+        } else {
+            for (int e = tid; e < KEYS * DMAX; e += THREADS) {
+                const int key = e / DMAX, c = e % DMAX;
+                const long long at = key_at[key];
+                const bool there = at >= 0 && c < D;
+                k_s[key * PITCH + c] = there ? to_f32(((const T*)p.pages)[at + c]) : 0.0f;
+                const float v = there ? to_f32(((const T*)p.pages)[at + v_offset + c]) : 0.0f;
+                v_s[key * DMAX + c] = v;
+                odd |= !(fabsf(v) < INFINITY);
+            }
+        }
+        odd = __syncthreads_or(odd);
+        // scores: a lane a key, the warp's four rows
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float* const k = k_s + lane * PITCH;
+#pragma unroll 8
+        for (int c = 0; c < DMAX; c += 4) {
+            const float4 k4 = *reinterpret_cast<const float4*>(k + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 q4 = *reinterpret_cast<const float4*>(q_s + (warp * 4 + i) * DMAX + c);
+                s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
+            }
+        }
+        const int key = base + lane, where = key_pos_s[lane];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = warp * 4 + i;
+            bool seen = where >= 0 && r < rows && (p.window <= 0 || where > pos_s[r] - p.window);
+            if (key >= length) seen = seen && ((mask_s[r][min((key - length) >> 5, MAX_WORDS - 1)] >> ((key - length) & 31)) & 1u) && (key - length) < p.words * 32;
+            const float x = seen ? s[i] * p.scale : -INFINITY;
+            const float m_new = fmaxf(m[i], warp_max(x));
+            const float e = seen ? expf(x - m_new) : 0.0f;
+            const float alpha = m[i] == -INFINITY ? 0.0f : expf(m[i] - m_new);
+            l[i] = l[i] * alpha + warp_sum(e);
+            m[i] = m_new;
+            p_s[r][lane] = e;
+            if (lane == 0) alpha_s[r] = alpha;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < RPT; ++r)
+#pragma unroll
+            for (int c = 0; c < COLS; ++c) acc[r][c] *= alpha_s[my_row + r];
+        if (odd) {
+            for (int j = 0; j < KEYS; ++j)
+#pragma unroll
+                for (int r = 0; r < RPT; ++r) {
+                    const float e = p_s[my_row + r][j];
+#pragma unroll
+                    for (int c = 0; c < COLS; ++c)
+                        if (e != 0.0f) acc[r][c] = fmaf(e, v_s[j * DMAX + my_col + c * 128], acc[r][c]);
+                }
+            continue;
+        }
+#pragma unroll 2
+        for (int j = 0; j < KEYS; j += 4) {
+            float v[4][COLS];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) v[i][c] = v_s[(j + i) * DMAX + my_col + c * 128];
+#pragma unroll
+            for (int r = 0; r < RPT; ++r) {
+                const float4 e = *reinterpret_cast<const float4*>(&p_s[my_row + r][j]);
+#pragma unroll
+                for (int c = 0; c < COLS; ++c) acc[r][c] = fmaf(e.w, v[3][c], fmaf(e.z, v[2][c], fmaf(e.y, v[1][c], fmaf(e.x, v[0][c], acc[r][c]))));
+            }
+        }
+    }
+    __syncthreads();
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { sum_s[warp * 4 + i] = l[i]; max_s[warp * 4 + i] = m[i]; }
+    }
+    __syncthreads();
+    const size_t all_rows = (size_t)p.tokens * p.heads;
+#pragma unroll
+    for (int r = 0; r < RPT; ++r) {
+        const int at = my_row + r;
+        if (at >= rows) continue;
+        const size_t row = (size_t)(start + (row0 + at) / G) * p.heads + kvh * G + (row0 + at) % G;
+        const float inv = sum_s[at] > 0.0f ? 1.0f / sum_s[at] : 0.0f;
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            const int col = my_col + c * 128;
+            if (col >= D) continue;
+            if (p.shares == 1) ((T*)p.out)[row * D + col] = from_f32<T>(acc[r][c] * inv);
+            else p.part_out[((size_t)share * all_rows + row) * D + col] = acc[r][c];
+        }
+        if (p.shares > 1 && my_col == 0) p.part_norm[(size_t)share * all_rows + row] = make_float2(max_s[at], sum_s[at]);
+    }
+}
+
+// a warp a row: the shares in their order
+template <typename T>
+__global__ void __launch_bounds__(THREADS) draft_join_kernel(DraftParams p) {
+    pdl_prologue();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y;
+    const int start = p.starts[seq], n = p.starts[seq + 1] - start;
+    const int at = blockIdx.x * (THREADS / 32) + warp;
+    if (at >= n * p.heads) return;
+    const size_t row = (size_t)start * p.heads + at, all_rows = (size_t)p.tokens * p.heads;
+    const int length = p.lengths[seq], keys = length + n - first_key(length, p.window) / KEYS * KEYS;
+    const int shares = min(p.shares, (keys + p.share - 1) / p.share);
+    float top = -INFINITY;
+    for (int s = lane; s < shares; s += 32) top = fmaxf(top, p.part_norm[s * all_rows + row].x);
+    top = warp_max(top);
+    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
+    if (top > -INFINITY) {
+        for (int s = 0; s < shares; ++s) {
+            const float2 norm = p.part_norm[s * all_rows + row];
+            if (norm.x == -INFINITY) continue;
+            const float w = expf(norm.x - top);
+            sum += norm.y * w;
+            const float* const o = p.part_out + (s * all_rows + row) * p.dim;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane + 32 * i < p.dim) acc[i] = fmaf(w, o[lane + 32 * i], acc[i]);
+        }
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    T* const out = (T*)p.out + row * p.dim;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < p.dim) out[lane + 32 * i] = from_f32<T>(acc[i] * inv);
+}
+
+template <typename T, int DMAX, bool PIECES>
+int launch_attention(const DraftParams& p, int sequences, cudaStream_t stream) {
+    constexpr int bytes = (ROWS * DMAX + KEYS * (DMAX + 4) + KEYS * DMAX) * 4;
+    static bool configured[MAX_DEVICES] = {};
+    const int d = device_index();
+    if (bytes > 40 * 1024 && !configured[d]) {
+        if (cudaFuncSetAttribute(draft_attention_kernel<T, DMAX, PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+            return check_launch("draft_attention: shared memory");
+        configured[d] = true;
+    }
+    launch_kernel(draft_attention_kernel<T, DMAX, PIECES>, dim3(p.shares, p.row_tiles * p.kv_heads, sequences), THREADS, bytes, stream, p);
+    return check_launch("draft_attention");
+}
+template <typename T, bool PIECES>
+int launch_attention(const DraftParams& p, int sequences, cudaStream_t stream) {
+    if (p.dim <= 32) return launch_attention<T, 32, PIECES>(p, sequences, stream);
+    if (p.dim <= 64) return launch_attention<T, 64, PIECES>(p, sequences, stream);
+    if (p.dim <= 128) return launch_attention<T, 128, PIECES>(p, sequences, stream);
+    return launch_attention<T, 256, PIECES>(p, sequences, stream);
+}
+
+template <typename T>
+int run_attention(const DraftParams& p, int sequences, int max_nodes, cudaStream_t stream) {
+    const bool pieces = p.dim % 4 == 0 && ((uintptr_t)p.pages & 15) == 0;
+    const int status = pieces ? launch_attention<T, true>(p, sequences, stream) : launch_attention<T, false>(p, sequences, stream);
+    if (status != MLB_OK || p.shares == 1) return status;
+    const int rows = THREADS / 32;
+    launch_kernel(draft_join_kernel<T>, dim3((max_nodes * p.heads + rows - 1) / rows, sequences), THREADS, 0, stream, p);
+    return check_launch("draft_join");
+}
+
+}  // namespace
+
+MLB_EXPORT int mlb_draft_masks(const int* parents, const int* starts, const int* lengths, int sequences, int words, int* masks, int* positions,
+                               int* places, int* error_flag, cudaStream_t stream) {
+    if (sequences < 0 || words <= 0 || words > MAX_WORDS) return fail(MLB_UNSUPPORTED_SIZE, "draft_masks: %d words a mask (at most %d)", words, MAX_WORDS);
+    if (sequences == 0) return MLB_OK;
+    launch_kernel(draft_masks_kernel, sequences, words * 32, 0, stream, parents, starts, lengths, words, masks, positions, places, error_flag);
+    return check_launch("draft_masks");
+}
+
+// scratch: shares > 1: [shares, T * NH] float2, then [shares, T * NH, D] fp32
+MLB_EXPORT int mlb_draft_attention(const void* q, const void* pages, void* out, int dtype, const int* starts, const int* lengths, const int* positions,
+                                   const int* masks, int words, const int* table, int max_blocks, int num_pages, int page_size, int tokens, int sequences,
+                                   int max_nodes, int heads, int kv_heads, int dim, float scale, int window, int share, int shares, void* scratch,
+                                   int* error_flag, cudaStream_t stream) {
+    if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || dim <= 0 || dim > 256)
+        return fail(MLB_UNSUPPORTED_SIZE, "draft_attention: heads %d/%d of %d elements", heads, kv_heads, dim);
+    if (words <= 0 || words > MAX_WORDS || max_nodes <= 0 || max_nodes > words * 32)
+        return fail(MLB_UNSUPPORTED_SIZE, "draft_attention: %d nodes in masks of %d words (at most %d)", max_nodes, words, MAX_WORDS);
+    if (num_pages <= 0 || page_size <= 0 || max_blocks <= 0 || tokens < 0 || sequences < 0 || window < 0) return fail(MLB_INVALID_ARGUMENT, "draft_attention: bad sizes");
+    if (share <= 0 || share % KEYS != 0 || shares <= 0 || (shares > 1 && !scratch)) return fail(MLB_INVALID_ARGUMENT, "draft_attention: bad shares");
+    const int group = heads / kv_heads, row_tiles = (max_nodes * group + ROWS - 1) / ROWS;
+    if (sequences > 65535 || row_tiles * kv_heads > 65535) return fail(MLB_UNSUPPORTED_SIZE, "draft_attention: too many sequences or rows");
+    if (tokens == 0 || sequences == 0) return MLB_OK;
+    DraftParams p{q, pages, out, starts, lengths, positions, masks, table, words, max_blocks, num_pages, page_size, heads, kv_heads, group, dim, window,
+                  row_tiles, share, shares, tokens, max_nodes, scale, nullptr, nullptr, error_flag};
+    p.part_norm = (float2*)scratch;
+    p.part_out = (float*)scratch + (size_t)2 * shares * tokens * heads;
+    if (dtype == MLB_F32) return run_attention<float>(p, sequences, max_nodes, stream);
+    if (dtype == MLB_BF16) return run_attention<__nv_bfloat16>(p, sequences, max_nodes, stream);
+    return fail(MLB_INVALID_ARGUMENT, "draft_attention: fp32 or bf16");
+}

@@ -41,6 +41,10 @@ def device_error_text(code: int) -> str:
     """What a non-zero device error flag means."""
     if code >= 10:
         return f"a bounded wait inside a tensor-memory kernel ran out (code {code}); the step's results are not valid"
+    if code == 3:
+        return "a drafted tree is not one (a parent that is no earlier node, or more nodes than the call was made for)"
+    if code == 4:
+        return "a beam's parent or state slot is out of range"
     return f"a kernel met a token without a valid page (code {code}): the block table and the request's length disagree"
 
 

@@ -1,0 +1,160 @@
+"""Trees of drafted tokens over the paged cache (`csrc/drafts.cu`, `csrc/cache_moves.cu`): masks and positions from the trees, their
+attention, and the branch that the model's choices accept.
+
+A step brings A sequences; sequence a has `lengths[a]` cached tokens and the nodes `starts[a] .. starts[a + 1]` of the step's T
+drafted ones.  Node i's `parents` entry is the index within the sequence of the node it continues, an earlier one, or -1; node 0
+is the token that the last step chose, which every other node continues.  Node i's keys and values go to place lengths[a] + i of
+the sequence's pages (`places`), while its position, which the rotation takes, is lengths[a] plus its depth.
+"""
+from __future__ import annotations
+
+from ctypes import c_float, c_int, c_void_p
+from typing import Optional
+
+import torch
+
+from . import build, ops
+from .build import KernelError
+from .cache_moves import PageMoves, need_current, need_on
+from .device import sm_count
+
+MAX_NODES = 256             # csrc/drafts.cu: nodes of a sequence
+ROWS, KEYS = 16, 32         # csrc/drafts.cu: rows (node, head of a group) and keys a CTA works on at a time
+SHARE_KEYS = 64             # keys below which a share is not cut further
+
+ops.register_signatures("drafts.cu", {
+    "mlb_draft_masks": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "mlb_draft_attention": [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                            c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
+})
+
+
+def _need_trees(device: int, starts: torch.Tensor, lengths: torch.Tensor) -> int:
+    need_on(device, starts, "starts", torch.int32, 1)
+    need_on(device, lengths, "lengths", torch.int32, 1)
+    if starts.shape[0] != lengths.shape[0] + 1:
+        raise KernelError("drafts: `starts` has one entry per sequence and one more")
+    return lengths.shape[0]
+
+
+def draft_masks(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, masks: torch.Tensor, positions: torch.Tensor,
+                places: Optional[torch.Tensor] = None, error_flag: Optional[torch.Tensor] = None) -> None:
+    """What a step's layers share: `masks` [T, words] int32, bit j of node i's row set for node i and every node above it (node
+    j of the same sequence), `positions` [T] = length + depth and `places` [T] = length + index.  `words` = ceil(most nodes of a sequence / 32), at
+    most 8.  A parent that is not an earlier node counts as none and raises the error flag; a sequence of more nodes than the masks hold
+    raises it too and is left out."""
+    device = parents.get_device()
+    need_on(device, parents, "parents", torch.int32, 1)
+    sequences = _need_trees(device, starts, lengths)
+    need_on(device, masks, "masks", torch.int32, 2)
+    need_on(device, positions, "positions", torch.int32, 1)
+    T = parents.shape[0]
+    if masks.shape[0] != T or positions.shape[0] != T or not 0 < masks.shape[1] <= MAX_NODES // 32:
+        raise KernelError(f"draft_masks: one row of 1 to {MAX_NODES // 32} words and one position per node")
+    if places is not None:
+        need_on(device, places, "places", torch.int32, 1)
+        if places.shape[0] != T:
+            raise KernelError("draft_masks: one place per node")
+    if error_flag is not None:
+        need_on(device, error_flag, "error_flag", torch.int32, 1)
+    need_current(device, "draft_masks")
+    L = ops.lib("drafts.cu")
+    build.check(L, L.mlb_draft_masks(parents.data_ptr(), starts.data_ptr(), lengths.data_ptr(), sequences, masks.shape[1], masks.data_ptr(), positions.data_ptr(),
+                                     ops._ptr(places), ops._ptr(error_flag), ops._stream()))
+
+
+def _shares(ctas: int, keys: int, sms: int):
+    """(keys a share, shares): the keys are split until two CTAs a multiprocessor have work, down to SHARE_KEYS."""
+    shares = max(1, min(-(-keys // SHARE_KEYS), 2 * sms // max(1, ctas)))
+    share = -(-(-(-keys // shares)) // KEYS) * KEYS
+    return share, -(-keys // share)
+
+
+def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor,
+                    masks: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
+                    window: Optional[int] = None, *, max_nodes: int, max_length: int, error_flag: Optional[torch.Tensor] = None) -> None:
+    """out[t, h] = softmax(scale q[t, h] . k) v over what node t sees: its sequence's cached tokens and the nodes of its mask, of both only
+    those of the last `window` positions where one is given.  A node that sees nothing gets zeros.
+
+    `q` and `out` [T, heads * D], `pages` [pages, 2, kv heads, page, D] of the same type (fp32 or bf16); `positions` and `masks` as `draft_masks`
+    makes them (any other mask over a sequence's nodes will do); `block_table` [sequences, blocks] int32.
+    `max_nodes`: the most nodes of a sequence, which the launch is sized for (a sequence of more raises the error flag).  `max_length`: the most keys
+    of a sequence, its nodes among them (how the work is cut; a longer sequence costs time only)."""
+    device = q.get_device()
+    tag = ops.dtype_tag(q)
+    need_on(device, q, "q", q.dtype, 2)
+    need_on(device, pages, "pages", q.dtype, 5)
+    need_on(device, out, "out", q.dtype, 2)
+    sequences = _need_trees(device, starts, lengths)
+    need_on(device, positions, "positions", torch.int32, 1)
+    need_on(device, masks, "masks", torch.int32, 2)
+    need_on(device, block_table, "block_table", torch.int32, 2)
+    T = q.shape[0]
+    num_pages, two, nkv, page_size, d = pages.shape
+    if two != 2 or nkv != num_kv_heads or d != head_dim:
+        raise KernelError(f"draft_attention: pages {tuple(pages.shape)} do not match the head geometry")
+    if num_kv_heads <= 0 or num_heads % num_kv_heads or not 0 < head_dim <= 256:
+        raise KernelError(f"draft_attention: heads {num_heads}/{num_kv_heads} of {head_dim}")
+    if q.shape[1] != num_heads * head_dim or out.shape != q.shape or positions.shape[0] != T or masks.shape[0] != T or block_table.shape[0] != sequences:
+        raise KernelError("draft_attention: shapes do not agree")
+    words = masks.shape[1]
+    if not 0 < words <= MAX_NODES // 32 or not 0 < max_nodes <= words * 32 or max_length < max_nodes:
+        raise KernelError(f"draft_attention: {max_nodes} nodes among {max_length} keys in masks of {words} words (at most {MAX_NODES // 32})")
+    if window is not None and window <= 0:
+        raise KernelError("draft_attention: a window has at least one key")
+    if error_flag is not None:
+        need_on(device, error_flag, "error_flag", torch.int32, 1)
+    if T == 0 or sequences == 0:
+        return
+    need_current(device, "draft_attention")
+    keys = min(max_length, window + max_nodes + KEYS) if window else max_length
+    row_tiles = -(-max_nodes * (num_heads // num_kv_heads) // ROWS)
+    share, shares = _shares(sequences * num_kv_heads * row_tiles, keys, sm_count(q.device))
+    scratch = ops.scratch(shares * T * num_heads * (head_dim + 2) * 4, q.device, "draft_attention") if shares > 1 else None
+    L = ops.lib("drafts.cu")
+    build.check(L, L.mlb_draft_attention(q.data_ptr(), pages.data_ptr(), out.data_ptr(), tag, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
+                                         masks.data_ptr(), words, block_table.data_ptr(), block_table.shape[1], num_pages, page_size, T, sequences, int(max_nodes),
+                                         num_heads, num_kv_heads, head_dim, float(scale), int(window or 0), share, shares, ops._ptr(scratch),
+                                         ops._ptr(error_flag), ops._stream()))
+
+
+def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor,
+                  counts: torch.Tensor, following: torch.Tensor, moves: Optional[PageMoves] = None, block_table: Optional[torch.Tensor] = None,
+                  error_flag: Optional[torch.Tensor] = None) -> None:
+    """The branch of each tree that the model confirms: from node 0, the lowest child whose token is the model's choice (`choices`, e.g.
+    `argmax_rows` of the nodes' logits) at its parent, and so on.  `path` [sequences, width >= most nodes] gets the nodes' indices (-1 behind them), `counts`
+    how many they are, `following` the model's choice behind the last one, which the next step's node 0 is.  With `moves` their rows of every pool
+    move from place lengths[a] + path[a, i] to lengths[a] + i, so that the cache holds the branch as if it had been decoded token by
+    token.  All int32.  A sequence without nodes gets a count of 0; one of more than `width` or 256 nodes raises the error flag."""
+    device = tokens.get_device()
+    for t, name in ((tokens, "tokens"), (parents, "parents"), (choices, "choices")):
+        need_on(device, t, name, torch.int32, 1)
+    sequences = _need_trees(device, starts, lengths)
+    need_on(device, path, "path", torch.int32, 2)
+    need_on(device, counts, "counts", torch.int32, 1)
+    need_on(device, following, "following", torch.int32, 1)
+    if parents.shape != tokens.shape or choices.shape != tokens.shape:
+        raise KernelError("accept_drafts: one token, parent and choice per node")
+    if path.shape[0] != sequences or path.shape[1] == 0 or counts.shape[0] != sequences or following.shape[0] != sequences:
+        raise KernelError("accept_drafts: one path, count and following token per sequence")
+    if error_flag is not None:
+        need_on(device, error_flag, "error_flag", torch.int32, 1)
+    groups = []
+    if moves is not None:
+        if not isinstance(moves, PageMoves):
+            raise KernelError("accept_drafts moves the storages of a PageMoves")
+        if block_table is None:
+            raise KernelError("accept_drafts: moving rows takes a block table")
+        need_on(device, block_table, "block_table", torch.int32, 2)
+        if block_table.shape[0] != sequences or (moves.groups and moves.device_index != device):
+            raise KernelError("accept_drafts: one row of the block table per sequence, and pools on the same device")
+        groups = moves.groups
+    if sequences == 0:
+        return
+    need_current(device, "accept_drafts")
+    L = ops.lib("cache_moves.cu")
+    trees = (tokens.data_ptr(), parents.data_ptr(), choices.data_ptr(), starts.data_ptr(), lengths.data_ptr(), sequences)
+    for i, (address, count, layout, _) in enumerate(groups or [(None, 0, (1, 1, 1, 1, 0, 0), None)]):
+        build.check(L, L.mlb_accept_drafts(address, count, *layout, *trees, ops._ptr(block_table), block_table.shape[1] if block_table is not None else 0,
+                                           path.data_ptr(), path.shape[1], counts.data_ptr(), following.data_ptr(), 1 if i == 0 else 0,
+                                           ops._ptr(error_flag), ops._stream()))

@@ -195,6 +195,11 @@ def part_sources():
             ("linear_attention.cu", {}), ("post_norm.cu", {}), ("streams.cu", {})]
 
 
+def continuation_sources():
+    """(source, defines) of the kernels for several continuations of a request: drafted trees and beams."""
+    return [("drafts.cu", {}), ("beams.cu", {}), ("cache_moves.cu", {})]
+
+
 def all_sources():
     """Every object the package can ask for with its default head sizes: what the build
     check compiles."""
@@ -203,7 +208,7 @@ def all_sources():
     for d in (32, 64, 128, 256):
         out += attention.mma_sources(d) + attention.tc_sources(d)
     from . import gemm_bf16, latent
-    return (out + gemm_bf16.sources() + [("gemv_noalloc.cu", {})] + part_sources()
+    return (out + gemm_bf16.sources() + [("gemv_noalloc.cu", {})] + part_sources() + continuation_sources()
             + latent.mma_sources(32, 8) + latent.mma_sources(256, 32) + latent.mma_sources(512, 64) + latent.tc_sources(512, 64))      # the widths of the presets
 
 
@@ -710,6 +715,17 @@ def on_side_stream(scratch=None):
 def second_stream():
     """(the second stream's handle while this thread's launches go there, else None; its `scratch`, or None)."""
     return getattr(_launch_on, "side", None), getattr(_launch_on, "scratch", None)
+
+
+def scratch(nbytes: int, device: torch.device, what: str) -> torch.Tensor:
+    """Memory for one call's own use between its launches: the tensor framework's, which takes it back in the order of the current stream.  A
+    launch on the second stream is not in that order, so there it is the step's (`on_side_stream(scratch)`)."""
+    side, step_scratch = second_stream()
+    if side is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if step_scratch is None:
+        raise KernelError(f"{what}: on the second stream it needs the step's scratch memory (on_side_stream(scratch))")
+    return step_scratch(nbytes)
 
 
 def stream_synchronize() -> None:
