@@ -21,12 +21,26 @@ from .device import sm_count
 MAX_NODES = 256             # csrc/drafts.cu: nodes of a sequence
 ROWS, KEYS = 16, 32         # csrc/drafts.cu: rows (node, head of a group) and keys a CTA works on at a time
 SHARE_KEYS = 64             # keys below which a share is not cut further
+TC_HEAD_DIMS, TC_KEYS, TC_ROWS = (64, 128), 128, 128        # csrc/drafts_tc.cu: keys a tile, rows of a stream (a CTA has two)
 
 ops.register_signatures("drafts.cu", {
     "mlb_draft_masks": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "mlb_draft_attention": [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
                             c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
 })
+ops.register_signatures("drafts_tc.cu", {
+    "mlb_draft_attention_tc": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                               c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
+})
+
+
+def tc_sources(head_dim: int):
+    return [("drafts_tc.cu", {"HEAD_DIM": head_dim})] if head_dim in TC_HEAD_DIMS else []
+
+
+def tc_supported(head_dim: int, page_size: int, group: int, scale: float) -> bool:
+    """What the tensor-core kernel takes (csrc/drafts_tc.cu): pages that divide a tile of keys, a group of heads that fits its rows."""
+    return (head_dim in TC_HEAD_DIMS and page_size >= 8 and page_size % 8 == 0 and TC_KEYS % page_size == 0 and group <= TC_ROWS and scale > 0.0)
 
 
 def _need_trees(device: int, starts: torch.Tensor, lengths: torch.Tensor) -> int:
@@ -107,8 +121,22 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     if T == 0 or sequences == 0:
         return
     need_current(device, "draft_attention")
+    group = num_heads // num_kv_heads
+    if q.dtype == torch.bfloat16 and tc_supported(head_dim, page_size, group, scale) and not (q.data_ptr() | pages.data_ptr() | out.data_ptr()) & 15:
+        keys = min(max_length, window + max_nodes + TC_KEYS) if window else max_length
+        tiles, pairs = -(-keys // TC_KEYS), -(-max_nodes // (2 * (TC_ROWS // group)))
+        shares = max(1, min(tiles, sm_count(q.device) // max(1, sequences * num_kv_heads * pairs)))
+        per = -(-tiles // shares)
+        shares = -(-tiles // per)
+        scratch = ops.scratch(shares * T * num_heads * (head_dim + 2) * 4, q.device, "draft_attention") if shares > 1 else None
+        L = ops.lib("drafts_tc.cu", {"HEAD_DIM": head_dim})
+        build.check(L, L.mlb_draft_attention_tc(q.data_ptr(), pages.data_ptr(), out.data_ptr(), starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
+                                                masks.data_ptr(), words, block_table.data_ptr(), block_table.shape[1], num_pages, page_size, T, sequences,
+                                                int(max_nodes), num_heads, num_kv_heads, float(scale), int(window or 0), per * TC_KEYS, shares, ops._ptr(scratch),
+                                                ops._ptr(error_flag), ops._stream()))
+        return
     keys = min(max_length, window + max_nodes + KEYS) if window else max_length
-    row_tiles = -(-max_nodes * (num_heads // num_kv_heads) // ROWS)
+    row_tiles = -(-max_nodes * group // ROWS)
     share, shares = _shares(sequences * num_kv_heads * row_tiles, keys, sm_count(q.device))
     scratch = ops.scratch(shares * T * num_heads * (head_dim + 2) * 4, q.device, "draft_attention") if shares > 1 else None
     L = ops.lib("drafts.cu")

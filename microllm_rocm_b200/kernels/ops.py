@@ -155,6 +155,11 @@ def lagged_latent_sources():
             [{"MLB_LAG_WARP": w} for w in (0, 1, 2, 5, 7)] + [{"MLB_SPIN_LIMIT": n} for n in (0, 1, 4)]]
 
 
+def lagged_draft_sources():
+    """And of the attention of drafted trees: both copying and issuing warps, and a softmax warp of each stream."""
+    return [("drafts_tc.cu", {"HEAD_DIM": 128, "MLB_LAG_WARP": w}) for w in (0, 1, 3, 8)]
+
+
 def lib(source: str, defines=None) -> ctypes.CDLL:
     if TEST_DEFINES.get(source):
         defines = {**(defines or {}), **TEST_DEFINES[source]}
@@ -197,7 +202,7 @@ def part_sources():
 
 def continuation_sources():
     """(source, defines) of the kernels for several continuations of a request: drafted trees and beams."""
-    return [("drafts.cu", {}), ("beams.cu", {}), ("cache_moves.cu", {})]
+    return [("drafts.cu", {}), ("drafts_tc.cu", {"HEAD_DIM": 64}), ("drafts_tc.cu", {"HEAD_DIM": 128}), ("beams.cu", {}), ("cache_moves.cu", {})]
 
 
 def all_sources():

@@ -549,3 +549,17 @@ def test_a_search_by_hand_beside_the_kernels():
         logits = weights[(state[:, 0].long() * 7 + chosen.long()) % V].contiguous()
     held = pool[table.long()].reshape(B, -1, 2)[:, :steps]
     assert held[..., 0].long().tolist() == lists and state[:, 0].long().tolist() == [sum(x) for x in lists] and int(error) == 0
+
+
+@pytest.mark.parametrize("lag", range(4))
+def test_attention_does_not_depend_on_which_warp_is_late(lag, monkeypatch):
+    """One warp of the tensor-core kernel sleeps at every turn of its loop: same bits, for streams that share the rows and for a row tile a stream."""
+    rng = random.Random(9)
+    steps = [Step(BF16, 6, 1, 128, 16, [900, 64], [random_tree(rng, 20), random_tree(rng, 3)], 1), Step(BF16, 6, 1, 128, 16, [700, 130], [random_tree(rng, 40), random_tree(rng, 64)], 2, 60)]
+    want = [s.run() for s in steps]
+    for s, w in zip(steps, want):
+        s.check(w)
+    source, defines = ops.lagged_draft_sources()[lag]
+    monkeypatch.setitem(ops.TEST_DEFINES, source, {k: v for k, v in defines.items() if k != "HEAD_DIM"})
+    for s, w in zip(steps, want):
+        assert torch.equal(s.run(), w) and int(s.error) == 0
