@@ -1,17 +1,22 @@
 // Attention of drafted trees over the paged bf16 cache on the fifth-generation tensor cores, heads of 64 or 128 (-DHEAD_DIM).  What a
-// row sees and how the shares of the keys are laid out is csrc/drafts.cu's; P is rounded to bf16 for the second product.
+// row sees is csrc/drafts.cu's; P is rounded to bf16 for the second product.
 //
-// A CTA takes one kv head of one sequence: the rows (node, head of the group) of up to 2 x floor(128 / group) nodes, and one share of
-// the keys in tiles of 128.  It holds two streams of work, each with four softmax warps (a thread a row), its own scores and its own
-// accumulator in tensor memory:
-//     rows for one tile of 128 or fewer:  both streams have the same rows; one takes the even key tiles, the other the odd ones, and they meet at the end
-//     more rows:                          a stream a row tile, both over every key tile, which is loaded once for the two
-// so that one stream's softmax runs beside the other's products.  Warps:
-//     warp 0      TMA: the queries (a box of heads x nodes, rows in the order node * group + head), then key and value tiles page by page
-//                 into a ring, in the order in which the products need them
+// An item is the rows (node, head of the group) of up to 2 x floor(128 / group) nodes of one sequence and kv head.  It has two streams of work, each
+// with four softmax warps (a thread a row), its own scores and its own accumulator in tensor memory:
+//     more nodes than one row tile holds:  a stream a row tile, both over every key tile of 128, which is loaded once for the two
+//     else: both streams have the same rows; one takes the even key tiles, the other the odd ones, and they meet at the end
+// so that one stream's softmax runs beside the other's products.
+//
+// The work of a call is a line of units (a row tile times a key tile), sequence after sequence, and every CTA takes an equal
+// stretch of it: the device counts the units from the lengths and trees as they are, so sequences of all lengths and trees of all sizes
+// fill the CTAs evenly.  A CTA's stretch may end in one item and begin in another; an item that lies in several CTAs leaves a partial result in each,
+// which a second kernel joins in order.
+//
+//     warp 0      TMA: key and value tiles page by page into a ring, in the order in which the products need them
+//     warp 3      TMA: a piece's queries (a box of heads x nodes, rows in the order node * group + head)
 //     warp 1      one thread issues tcgen05.mma: S = Q K^T; O += P V with P in tensor memory.  P overwrites the scores it was made of; the next scores of a stream
 //                 are issued behind the product that reads P, so "scores are there" also says that the accumulator is (the tensor pipe runs in order)
-//     warps 2-9   softmax of stream (warp - 2) / 4: mask in the tiles that need one, running maximum and sum in fp32 with base-2
+//     warps 4-11  softmax of stream (warp - 4) / 4: mask in the tiles that need one, running maximum and sum in fp32 with base-2
 //                 exponentials, the accumulator rescaled only when a row's maximum has grown by 2^8
 // In tiles that not every row sees alike the value rows are looked through: one that holds a number which is not finite is cleared for the product (0 * NaN
 // would reach rows that do not see it) and the rows that do see it become NaN; value rows that nobody sees are cleared too.
@@ -41,9 +46,13 @@ constexpr int ROW_BYTES = 128;               // one swizzle span
 constexpr int Q_BYTES = SPANS * BM * ROW_BYTES;
 constexpr int KV_BYTES = SPANS * BN * ROW_BYTES;
 constexpr int SLOTS = D == 128 ? 5 : 8;
-constexpr int SMEM_BYTES = 2 * Q_BYTES + SLOTS * KV_BYTES + 1024;
-static_assert(SMEM_BYTES + 512 <= 227 * 1024, "a CTA's shared memory, its barriers among it");
-constexpr int THREADS = 320;
+constexpr int SHARED_BYTES = 3072;           // barriers and what the warps tell one another, behind the tiles
+constexpr int SMEM_BYTES = 2 * Q_BYTES + SLOTS * KV_BYTES + SHARED_BYTES;
+static_assert(SMEM_BYTES <= 227 * 1024, "a CTA's shared memory");
+constexpr int THREADS = 384;
+// 384 threads start with 168 registers each; the softmax warps hold a whole row of scores
+constexpr int FEW_REGISTERS = 80, MANY_REGISTERS = 208;
+static_assert(128 * FEW_REGISTERS + 256 * MANY_REGISTERS <= THREADS * 168, "no more than the launch has");
 constexpr int STREAM_COLS = 256;             // tensor memory of a stream: scores (then P as bf16 pairs) [0, 128), accumulator [128, 128 + D)
 constexpr int TMEM_COLS = 2 * STREAM_COLS;
 constexpr int O_COL = BN;
@@ -52,6 +61,10 @@ constexpr int MAX_PAGES_PER_TILE = 16;
 constexpr int MAX_WORDS = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.0f;
+#ifndef V_CHUNK
+#define V_CHUNK 32
+#endif
+constexpr int CHUNK = V_CHUNK;
 
 struct TcParams {
     __nv_bfloat16* out;             // [T, NH * D]
@@ -61,12 +74,13 @@ struct TcParams {
     const int* masks;               // [T, words]
     const int* table;               // [A, max_blocks]
     int words, max_blocks, num_pages, page_size, pages_per_tile;
-    int heads, kv_heads, group, tile_nodes, pairs, window, max_nodes;
-    int share;                      // keys of a share, a multiple of BN
-    int shares, tokens;
+    int heads, kv_heads, group, tile_nodes, row_tiles, window, max_nodes;      // row_tiles: of a sequence of max_nodes
+    int stretch;                    // units of a CTA at least
+    int ctas, sequences, tokens;
     float scale_log2;
-    float* part_out;                // [shares, T * NH, D]
-    float2* part_norm;              // [shares, T * NH]
+    float* part_out;                // [ctas, 2, 2, D, BM]: of the item that a CTA's stretch begins in, and of the one that it ends in; a column's rows together
+    float2* part_norm;              // [ctas, 2, 2, BM]
+    int* line;                      // [2 + sequences]: units a CTA, units an item begins with, then every sequence's first unit (what the join asks for)
     int* error_flag;
 };
 
@@ -165,6 +179,18 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
                    "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
                  : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -232,465 +258,701 @@ __device__ __forceinline__ unsigned bit_range(int from, int to) {
     return upper & ~lower;
 }
 
-// the keys of a sequence that a CTA's share holds, in tiles
-struct Span {
-    int lo, total, first, count;    // the first key any node may see, all keys, the first tile and how many
+// A sequence's part of the line.
+struct Sequence {
+    int token0, n, length, lo, first, tiles, row_tiles;    // lo: the first key any node may see; first: its tile
+    __device__ __forceinline__ int items() const { return (row_tiles + 1) >> 1; }       // of a head
+    __device__ __forceinline__ int units(int kv_heads, int lead) const { return kv_heads * (tiles * row_tiles + lead * items()); }
 };
-__device__ __forceinline__ Span span_of(const TcParams& p, int length, int n, int share) {
-    Span s;
-    s.lo = p.window > 0 ? max(0, length - p.window + 1) : 0;
-    s.total = length + n;
-    const int per = p.share / BN;
-    s.first = s.lo / BN + share * per;
-    const int tiles = (s.total + BN - 1) / BN - s.first;
-    s.count = max(0, share == p.shares - 1 ? tiles : min(tiles, per));
+__device__ __forceinline__ Sequence sequence_at(const TcParams& p, int a) {
+    Sequence s;
+    s.token0 = p.starts[a];
+    s.n = min(p.starts[a + 1] - s.token0, p.max_nodes);
+    s.length = p.lengths[a];
+    s.lo = p.window > 0 ? max(0, s.length - p.window + 1) : 0;
+    s.first = s.lo / BN;
+    s.tiles = s.n > 0 ? (s.length + s.n + BN - 1) / BN - s.first : 0;
+    s.row_tiles = s.n > 0 ? (s.n + p.tile_nodes - 1) / p.tile_nodes : 0;
     return s;
 }
 
+// How the line is cut, by one whole warp: units a CTA, and for this CTA its stretch, the sequence that it begins in and that one's first unit.  CTA 0
+// leaves all sequences' first units for the join.
+//
+// Every item begins with `lead` units that stand for no work: what it costs a CTA to end one item (results out, accumulators free) and begin another is about
+// four turns' time, and without them the CTAs that hold an item's end and the next one's beginning were the last by a fifth of the kernel's time.  Short
+// stretches, where a call waits for the first tile and not for the last CTA, take less.
+constexpr int MOST_LEAD = 6;
+struct Cut {
+    int stretch, lead, unit, end, a, base;
+};
+__device__ __forceinline__ Cut cut_line(const TcParams& p, int lane) {
+    auto sequence = [&](int a) {
+        if (a < p.sequences) return sequence_at(p, a);
+        Sequence none = {};
+        return none;
+    };
+    const Sequence mine = sequence(lane);                 // of the first 32 sequences, most calls' only ones
+    int total = mine.units(p.kv_heads, 0), items = mine.items() * p.kv_heads;
+    for (int a = lane + 32; a < p.sequences; a += 32) {
+        const Sequence s = sequence(a);
+        total += s.units(p.kv_heads, 0);
+        items += s.items() * p.kv_heads;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    items = __reduce_add_sync(0xffffffffu, items);
+    Cut c;
+    c.lead = min(MOST_LEAD, (total + p.ctas - 1) / p.ctas / 2);
+    total += items * c.lead;
+    c.stretch = max(p.stretch, (total + p.ctas - 1) / p.ctas);
+    c.unit = min((int)blockIdx.x * c.stretch, total);
+    c.end = min(c.unit + c.stretch, total);
+    c.a = p.sequences;
+    c.base = 0;
+    if (blockIdx.x == 0 && lane == 0 && p.line) {
+        p.line[0] = c.stretch;
+        p.line[1] = c.lead;
+    }
+    int base = 0;
+    for (int a0 = 0; a0 < p.sequences; a0 += 32) {
+        const int units = (a0 ? sequence(a0 + lane) : mine).units(p.kv_heads, c.lead);
+        int sum = units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += other;
+        }
+        if (blockIdx.x == 0 && p.line && a0 + lane < p.sequences) p.line[2 + a0 + lane] = base + sum - units;
+        const unsigned hit = __ballot_sync(0xffffffffu, units > 0 && base + sum > c.unit);
+        if (hit && c.a == p.sequences) {
+            const int at = __ffs(hit) - 1;
+            c.a = a0 + at;
+            c.base = base + __shfl_sync(0xffffffffu, sum - units, at);
+            if (blockIdx.x != 0 || !p.line) break;
+        }
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return c;
+}
+
+// One item of a sequence, and the key tiles of it that the units [from, to) are.
+struct Item {
+    int kvh, node0, begin, work, end;    // its units: begin .. work stand for no tile
+    bool paired;
+};
+__device__ __forceinline__ Item item_of(const TcParams& p, const Sequence& s, int base, int lead, int kvh, int pair) {
+    Item i;
+    i.kvh = kvh;
+    i.node0 = pair * 2 * p.tile_nodes;
+    i.paired = s.row_tiles - 2 * pair >= 2;
+    i.begin = base + kvh * s.units(1, lead) + pair * (2 * s.tiles + lead);
+    i.work = i.begin + lead;
+    i.end = i.work + (i.paired ? 2 : 1) * s.tiles;
+    return i;
+}
+__device__ __forceinline__ Item item_at(const TcParams& p, const Sequence& s, int base, int lead, int unit) {
+    const int per_head = s.units(1, lead), at = unit - base, kvh = at / per_head;
+    return item_of(p, s, base, lead, kvh, (at - kvh * per_head) / (2 * s.tiles + lead));
+}
+// a unit of an item as a key tile: a cut between the two units of a paired item's tile counts the tile to the part in front
+__device__ __forceinline__ int tile_of(const Item& i, int unit) {
+    const int at = max(0, unit - i.work);
+    return i.paired ? (at + 1) >> 1 : at;
+}
+
+// What a CTA walks through: every role has its own.
+struct Walk {
+    int unit, end, a, base, known;       // known: the sequence that `s` is of
+    Sequence s;
+    Item item;
+    int tile, n_tiles, part, parts;      // first key tile (from s.first), how many, which part of how many
+    __device__ __forceinline__ bool next(const TcParams& p, int stretch, int lead) {
+        while (unit < end) {
+            while (true) {
+                if (a != known) s = sequence_at(p, a);
+                known = a;
+                const int units = s.units(p.kv_heads, lead);
+                if (unit < base + units) break;
+                base += units;
+                ++a;
+            }
+            item = item_at(p, s, base, lead, unit);
+            const int to = min(end, item.end);
+            tile = tile_of(item, unit);
+            n_tiles = tile_of(item, to) - tile;
+            part = unit / stretch - item.begin / stretch;
+            parts = (item.end - 1) / stretch - item.begin / stretch + 1;
+            unit = to;
+            if (n_tiles > 0) return true;
+        }
+        return false;
+    }
+};
+
+struct Shared {
+    unsigned long long q_full, q_empty, slot_full[SLOTS], slot_empty[SLOTS], s_full[2], p_full[2], o_full[2], v_checked[3], norms_there, o_read;
+    uint32_t tmem_base;
+    int failed, unit, end, a, base, stretch, lead, pieces, issued;      // pieces, issued: whose copies were asked for
+    Sequence s;
+    unsigned odd[3][2][4];               // [streams, or both][turn & 1]: which of a tile's value rows are not finite
+    float2 norm[2 * BM];                 // the rows' maxima and sums, for streams that share the rows
+};
+static_assert(sizeof(Shared) <= SHARED_BYTES, "what the warps tell one another");
+
 __global__ void __launch_bounds__(THREADS, 1)
 draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, TcParams p) {
-    pdl_launch_dependents();
-    extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(8) unsigned long long q_full, slot_full[SLOTS], slot_empty[SLOTS], s_full[2], p_full[2], o_full[2], v_checked[2], norms_there;
-    __shared__ uint32_t tmem_base_s;
-    __shared__ int failed_s;
-    __shared__ unsigned odd_s[2][2][4];           // [stream][turn & 1]: which of a tile's value rows are not finite
-
+    extern __shared__ __align__(1024) unsigned char smem_dyn[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;     // the swizzle pattern wants 1024-byte alignment
+    const uint32_t base = smem_u32(smem_dyn);
     const uint32_t q_s = base;
     const uint32_t ring_s = q_s + 2 * Q_BYTES;
-    // the rows' maxima and sums, for streams that share the rows: there the second query tile's place is free
-    float2* const norm_s = reinterpret_cast<float2*>(smem_dyn + (base - smem_u32(smem_dyn)) + Q_BYTES);
+    Shared& sh = *reinterpret_cast<Shared*>(smem_dyn + 2 * Q_BYTES + SLOTS * KV_BYTES);
 
-    pdl_wait();                  // (the sequence's extents may be the kernel before's)
-    // ---- what this CTA works on (uniform)
-    const int share = blockIdx.x, seq = blockIdx.z;
-    const int kvh = blockIdx.y / p.pairs, pair = blockIdx.y % p.pairs;
-    const int token0 = p.starts[seq], n = p.starts[seq + 1] - token0, length = p.lengths[seq];
-    const int node0 = pair * 2 * p.tile_nodes;                       // the first node of this CTA's rows
-    if (n <= node0) return;
-    if (n > p.max_nodes && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 3);
-    const Span span = span_of(p, length, n, share);
-    if (span.count == 0) return;                                     // (never share 0; the join knows)
-    const int n_tiles = span.count;
-    const bool paired = n - node0 > p.tile_nodes;                    // a row tile a stream; else the streams share the key tiles
-    // stream s: its tiles are t = t0, t0 + dt, ..
-    const int dt = paired ? 1 : 2;
-
+    if (warp == 3 && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"(lane ? &map_kv : &map_q) : "memory");
     if (threadIdx.x == 0) {
-        mbar_init(smem_u32(&q_full), 1);
+        mbar_init(smem_u32(&sh.q_full), 1);
+        mbar_init(smem_u32(&sh.q_empty), 1);
         for (int s = 0; s < SLOTS; ++s) {
-            mbar_init(smem_u32(&slot_full[s]), 1);
-            mbar_init(smem_u32(&slot_empty[s]), 1);
+            mbar_init(smem_u32(&sh.slot_full[s]), 1);
+            mbar_init(smem_u32(&sh.slot_empty[s]), 1);
         }
         for (int s = 0; s < 2; ++s) {
-            mbar_init(smem_u32(&s_full[s]), 1);
-            mbar_init(smem_u32(&p_full[s]), 4);          // one arrival per softmax warp
-            mbar_init(smem_u32(&o_full[s]), 1);
-            mbar_init(smem_u32(&v_checked[s]), paired ? 8 : 4);
+            mbar_init(smem_u32(&sh.s_full[s]), 1);
+            mbar_init(smem_u32(&sh.p_full[s]), 4);          // one arrival per softmax warp
+            mbar_init(smem_u32(&sh.o_full[s]), 1);
+            mbar_init(smem_u32(&sh.v_checked[s]), 4);
         }
-        mbar_init(smem_u32(&norms_there), 8);
-        failed_s = 0;
+        mbar_init(smem_u32(&sh.v_checked[2]), 8);
+        mbar_init(smem_u32(&sh.norms_there), 8);
+        mbar_init(smem_u32(&sh.o_read), 8);
+        sh.failed = (base & 1023u) ? 1 : 0;                 // the swizzle pattern wants 1024-byte alignment
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
+    pdl_wait();                  // queries, this step's keys, and the sequences' extents may be the kernel before's
+    // The tensor memory is taken between the wait and the next kernel's early start: neither a kernel in front that still needs some nor one
+    // behind that already waits for this one can stand in the way, or be stood in the way of.
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(&tmem_base_s)), "r"((uint32_t)TMEM_COLS) : "memory");
+                     ::"r"(smem_u32(&sh.tmem_base)), "r"((uint32_t)TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (warp == 2) {
+        const Cut cut = cut_line(p, lane);
+        const Sequence s = sequence_at(p, min(cut.a, p.sequences - 1));
+        if (lane == 0) {
+            sh.s = s;
+            sh.unit = cut.unit;
+            sh.end = cut.end;
+            sh.a = cut.a;
+            sh.base = cut.base;
+            sh.stretch = cut.stretch;
+            sh.lead = cut.lead;
+        }
+    } else if (warp == 4 && blockIdx.x == 0) {
+        for (int a = lane; a < p.sequences; a += 32)
+            if (p.starts[a + 1] - p.starts[a] > p.max_nodes && p.error_flag) atomicExch(p.error_flag, 3);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_base = tmem_base_s;
+    pdl_launch_dependents();
+    const uint32_t tmem_base = sh.tmem_base;
+    const int stretch = sh.stretch, lead = sh.lead;
+    Walk walk;
+    walk.unit = sh.failed ? sh.end : sh.unit;
+    walk.end = sh.end;
+    walk.a = sh.a;
+    walk.base = sh.base;
+    walk.known = sh.a;
+    walk.s = sh.s;
+    if (sh.failed && threadIdx.x == 0 && p.error_flag) atomicCAS(p.error_flag, 0, 40);
 
-    // Ring items in order of need.  Shared key tiles: K0 K1 V0 K2 V1 K3 ..; a row tile a stream: K0 V0 K1 V1 ..
-    // The items walk like this for all who count them: prologue K(0 .. dt - 1), then for every t: V(t), K(t + dt).
-    const int prologue = min(dt, n_tiles);
-    int issued = 0;
-
-    if (warp == 0) {
-        // ------------------------------------------------------------------ producer (whole warp)
-        if (lane == 0) {
-            const int boxes = paired ? 2 : 1;
-            mbar_expect_tx(smem_u32(&q_full), boxes * SPANS * p.tile_nodes * p.group * ROW_BYTES);
-            for (int b = 0; b < boxes; ++b)
+    // Ring items in order of need, piece after piece.  Shared key tiles: K0 K1 V0 K2 V1 K3 ..; a row tile a stream: K0 V0 K1 V1 ..: K(0 .. dt - 1)
+    // first, then for every t: V(t), K(t + dt).  A piece of n key tiles is 2 n items.
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FEW_REGISTERS));
+        if (warp == 0) {
+            // -------------------------------------------------------------- keys and values (whole warp)
+            bool ok = true;
+            int issued = 0;
+            while (ok && walk.next(p, stretch, lead)) {
+                const Sequence& s = walk.s;
+                const int dt = walk.item.paired ? 1 : 2, n_tiles = walk.n_tiles;
+                const int* table = p.table + (size_t)walk.a * p.max_blocks;
+                // lane g: the page of block g of a tile.  Two key tiles' pages are on their way ahead of their use.
+                auto lookup = [&](int t) {
+                    const int block = (s.first + walk.tile + t) * p.pages_per_tile + lane;
+                    return t < n_tiles && lane < p.pages_per_tile && block < p.max_blocks ? __ldg(table + block) : -1;
+                };
+                auto load = [&](int t, int page, int is_v) {
+                    lag_point();
+                    const int slot = issued % SLOTS;
+                    if (issued >= SLOTS) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.slot_empty[slot]), ((issued / SLOTS) - 1) & 1, p.error_flag, 42)) != 0;
+                    if (!ok) return;
+                    const uint32_t bar = smem_u32(&sh.slot_full[slot]);
+                    if (lane == 0) mbar_expect_tx(bar, KV_BYTES);
+                    __syncwarp();
+                    if (lane < p.pages_per_tile) {
+                        if (page < 0 || page >= p.num_pages) {
+                            // a page that holds a key some row may see has to exist; the others are masked
+                            const int first_key = ((s.first + walk.tile + t) * p.pages_per_tile + lane) * p.page_size;
+                            if (first_key < s.length + s.n && first_key + p.page_size > s.lo && p.error_flag) atomicExch(p.error_flag, 2);
+                            page = 0;
+                        }
+                        const int row = ((page * 2 + is_v) * p.kv_heads + walk.item.kvh) * p.page_size;
+                        const uint32_t dst = ring_s + slot * KV_BYTES + lane * p.page_size * ROW_BYTES;
 #pragma unroll
-                for (int s = 0; s < SPANS; ++s)
-                    tma_load_3d(q_s + b * Q_BYTES + s * BM * ROW_BYTES, &map_q, s * 64, kvh * p.group, token0 + node0 + b * p.tile_nodes, smem_u32(&q_full));
-        }
-        const int* table = p.table + (size_t)seq * p.max_blocks;
-        auto lookup = [&](int tile) {                     // lane g: the page of block g of a tile
-            const int block = (span.first + tile) * p.pages_per_tile + lane;
-            return (lane < p.pages_per_tile && block < p.max_blocks) ? __ldg(table + block) : -1;
-        };
-        bool ok = true;
-        int item = 0;                                     // = issued
-        auto load = [&](int tile, int is_v) {
-            lag_point();
-            int page = lookup(tile);
-            const int slot = item % SLOTS;
-            if (item >= SLOTS) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&slot_empty[slot]), ((item / SLOTS) - 1) & 1, p.error_flag, 41)) != 0;
-            if (!ok) return;
-            const uint32_t bar = smem_u32(&slot_full[slot]);
-            if (lane == 0) mbar_expect_tx(bar, KV_BYTES);
-            __syncwarp();
-            if (lane < p.pages_per_tile) {
-                if (page < 0 || page >= p.num_pages) {
-                    // a page that holds a key some row may see has to exist; the others are masked
-                    const int first_key = ((span.first + tile) * p.pages_per_tile + lane) * p.page_size;
-                    if (first_key < span.total && first_key + p.page_size > span.lo && p.error_flag) atomicExch(p.error_flag, 2);
-                    page = 0;
+                        for (int c = 0; c < SPANS; ++c) tma_load_2d(dst + c * BN * ROW_BYTES, &map_kv, c * 64, row, bar);
+                    }
+                    ++issued;
+                };
+                int page = lookup(0), next = lookup(1), after = lookup(2);       // of tiles t, t + 1, t + 2
+                load(0, page, 0);
+                if (ok && dt == 2 && n_tiles > 1) load(1, next, 0);
+                for (int t = 0; t < n_tiles && ok; ++t) {
+                    const int third = lookup(t + 3);
+                    load(t, page, 1);
+                    if (ok && t + dt < n_tiles) load(t + dt, dt == 1 ? next : after, 0);
+                    page = next;
+                    next = after;
+                    after = third;
                 }
-                const int row = ((page * 2 + is_v) * p.kv_heads + kvh) * p.page_size;
-                const uint32_t dst = ring_s + slot * KV_BYTES + lane * p.page_size * ROW_BYTES;
-#pragma unroll
-                for (int s = 0; s < SPANS; ++s) tma_load_2d(dst + s * BN * ROW_BYTES, &map_kv, s * 64, row, bar);
             }
-            ++item;
-            issued = item;
-        };
-        for (int t = 0; t < prologue && ok; ++t) load(t, 0);
-        for (int t = 0; t < n_tiles && ok; ++t) {
-            load(t, 1);
-            if (ok && t + dt < n_tiles) load(t + dt, 0);
-        }
-        if (!ok && lane == 0) failed_s = 1;
-    } else if (warp == 1) {
-        // ------------------------------------------------------------------ MMA issue: the warp walks converged, one lane issues
-        const uint32_t idesc_qk = idesc(BN, false), idesc_pv = idesc(D, true);
-        auto wait_warp = [&](unsigned long long* bar, uint32_t parity, int code) {
-            return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, p.error_flag, code)) != 0;
-        };
-        bool ok = n_tiles == 0 || wait_warp(&q_full, 0, 42);
-        int item = 0;                                      // ring items are consumed in the order they were loaded
-        auto full = [&](int i, int code) { return wait_warp(&slot_full[i % SLOTS], (i / SLOTS) & 1, code); };
-        auto issue_qk = [&](int s, int i, bool last_use) { // stream s's scores from ring item i
-            const uint32_t kb = ring_s + (i % SLOTS) * KV_BYTES, qb = q_s + (paired ? s * Q_BYTES : 0);
-            if (elect_one()) {
+            if (!ok && lane == 0) sh.failed = 1;
+            if (lane == 0) sh.issued = issued;
+        } else if (warp == 3) {
+            // -------------------------------------------------------------- queries: a piece ahead of the products at most
+            bool ok = true;
+            int pieces = 0;
+            for (; walk.next(p, stretch, lead); ++pieces) {
+                if (pieces > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.q_empty), (pieces - 1) & 1, p.error_flag, 41)) != 0;
+                if (!ok) break;
+                if (lane == 0) {
+                    const int boxes = walk.item.paired ? 2 : 1;
+                    mbar_expect_tx(smem_u32(&sh.q_full), boxes * SPANS * p.tile_nodes * p.group * ROW_BYTES);
+                    for (int b = 0; b < boxes; ++b)
 #pragma unroll
-                for (int ks = 0; ks < D / 16; ++ks) {
-                    const uint32_t off = (ks / 4) * (BM * ROW_BYTES) + (ks % 4) * 32;
-                    umma(tmem_base + (uint32_t)(s * STREAM_COLS), desc_k_major(qb + off), desc_k_major(kb + off), idesc_qk, ks > 0);
+                        for (int c = 0; c < SPANS; ++c)
+                            tma_load_3d(q_s + b * Q_BYTES + c * BM * ROW_BYTES, &map_q, c * 64, walk.item.kvh * p.group, walk.s.token0 + walk.item.node0 + b * p.tile_nodes,
+                                        smem_u32(&sh.q_full));
                 }
-                if (last_use) umma_commit(smem_u32(&slot_empty[i % SLOTS]));
-                umma_commit(smem_u32(&s_full[s]));
+                __syncwarp();
             }
-            __syncwarp();
-        };
-        auto issue_pv = [&](int s, int i, bool first, bool last, bool last_use) {
-            const uint32_t vb = ring_s + (i % SLOTS) * KV_BYTES;
-            if (elect_one()) {
+            if (!ok && lane == 0) sh.failed = 1;
+            if (lane == 0) sh.pieces = pieces;
+        } else if (warp == 1) {
+            // -------------------------------------------------------------- MMA issue: the warp walks converged, one lane issues
+            const uint32_t idesc_qk = idesc(BN, false), idesc_pv = idesc(D, true);
+            auto wait_warp = [&](unsigned long long* bar, uint32_t parity, int code) {
+                return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, p.error_flag, code)) != 0;
+            };
+            bool ok = true;
+            int item = 0, piece = 0;                           // ring items are consumed in the order they were loaded
+            int turn[2] = {0, 0};                              // P's of each stream so far
+            auto full = [&](int i, int code) { return wait_warp(&sh.slot_full[i % SLOTS], (i / SLOTS) & 1, code); };
+            while (ok && walk.next(p, stretch, lead)) {
+                const bool paired = walk.item.paired;
+                const int n_tiles = walk.n_tiles;
+                auto issue_qk = [&](int s, int i, bool last_use, bool last) {       // stream s's scores from ring item i
+                    const uint32_t kb = ring_s + (i % SLOTS) * KV_BYTES, qb = q_s + (paired ? s * Q_BYTES : 0);
+                    if (elect_one()) {
 #pragma unroll
-                for (int ks = 0; ks < BN / 16; ++ks)           // 16 keys = 8 columns of P
-                    umma_ts(tmem_base + (uint32_t)(s * STREAM_COLS + O_COL), tmem_base + (uint32_t)(s * STREAM_COLS + ks * 8),
-                            desc_mn_major(vb + ks * 16 * ROW_BYTES, BN * ROW_BYTES), idesc_pv, (!first || ks > 0) ? 1u : 0u);
-                if (last_use) umma_commit(smem_u32(&slot_empty[i % SLOTS]));
-                if (last) umma_commit(smem_u32(&o_full[s]));
-            }
-            __syncwarp();
-        };
-        if (paired) {
-            if (ok && n_tiles > 0) {
-                ok = full(item, 43);
-                if (ok) {
-                    issue_qk(0, item, false);
-                    issue_qk(1, item, true);
+                        for (int ks = 0; ks < D / 16; ++ks) {
+                            const uint32_t off = (ks / 4) * (BM * ROW_BYTES) + (ks % 4) * 32;
+                            umma(tmem_base + (uint32_t)(s * STREAM_COLS), desc_k_major(qb + off), desc_k_major(kb + off), idesc_qk, ks > 0);
+                        }
+                        if (last_use) umma_commit(smem_u32(&sh.slot_empty[i % SLOTS]));
+                        if (last) umma_commit(smem_u32(&sh.q_empty));
+                        umma_commit(smem_u32(&sh.s_full[s]));
+                    }
+                    __syncwarp();
+                };
+                auto issue_pv = [&](int s, int i, bool first, bool last, bool last_use) {
+                    const uint32_t vb = ring_s + (i % SLOTS) * KV_BYTES;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int ks = 0; ks < BN / 16; ++ks)           // 16 keys = 8 columns of P
+                            umma_ts(tmem_base + (uint32_t)(s * STREAM_COLS + O_COL), tmem_base + (uint32_t)(s * STREAM_COLS + ks * 8),
+                                    desc_mn_major(vb + ks * 16 * ROW_BYTES, BN * ROW_BYTES), idesc_pv, (!first || ks > 0) ? 1u : 0u);
+                        if (last_use) umma_commit(smem_u32(&sh.slot_empty[i % SLOTS]));
+                        if (last) umma_commit(smem_u32(&sh.o_full[s]));
+                    }
+                    __syncwarp();
+                };
+                ok = wait_warp(&sh.q_full, piece & 1, 43);
+                if (!ok) break;
+                ++piece;
+                const int dt = paired ? 1 : 2;
+                for (int t = 0; t < min(dt, n_tiles) && ok; ++t) {
+                    ok = full(item, 44);
+                    if (!ok) break;
+                    if (paired) {
+                        issue_qk(0, item, false, false);
+                        issue_qk(1, item, true, n_tiles == 1);
+                    } else {
+                        issue_qk(t, item, true, t + 1 == n_tiles);
+                    }
                     ++item;
                 }
-            }
-            for (int t = 0; t < n_tiles && ok; ++t) {
-                lag_point();
-                const bool last = t + 1 == n_tiles;
-                ok = wait_warp(&p_full[0], t & 1, 44) && full(item, 45);
-                if (!ok) break;
-                tc_fence_after();
-                issue_pv(0, item, t == 0, last, false);
-                if (!last) {
-                    ok = full(item + 1, 46);
+                for (int t = 0; t < n_tiles && ok; ++t) {
+                    lag_point();
+                    const bool more = t + dt < n_tiles, last = t + dt >= n_tiles;
+                    const int s0 = paired ? 0 : t & 1;
+                    ok = wait_warp(&sh.p_full[s0], turn[s0] & 1, 45) && full(item, 46);
                     if (!ok) break;
-                    issue_qk(0, item + 1, false);
-                }
-                ok = wait_warp(&p_full[1], t & 1, 47);
-                if (!ok) break;
-                tc_fence_after();
-                issue_pv(1, item, t == 0, last, true);
-                if (!last) issue_qk(1, item + 1, true);
-                item += 2;
-            }
-        } else {
-            for (int t = 0; t < prologue && ok; ++t) {
-                ok = full(item, 48);
-                if (!ok) break;
-                issue_qk(t, item, true);
-                ++item;
-            }
-            for (int t = 0; t < n_tiles && ok; ++t) {
-                lag_point();
-                const int s = t & 1;
-                ok = wait_warp(&p_full[s], (t >> 1) & 1, 49) && full(item, 50);
-                if (!ok) break;
-                tc_fence_after();
-                issue_pv(s, item, t < 2, t + 2 >= n_tiles, true);
-                ++item;
-                if (t + 2 < n_tiles) {
-                    ok = full(item, 51);
-                    if (!ok) break;
-                    issue_qk(s, item, true);
-                    ++item;
+                    ++turn[s0];
+                    tc_fence_after();
+                    issue_pv(s0, item, t < dt, last, !paired);
+                    if (more) {
+                        ok = full(item + 1, 47);
+                        if (!ok) break;
+                        issue_qk(s0, item + 1, !paired, !paired && t + dt + 1 == n_tiles);
+                    }
+                    if (paired) {
+                        ok = wait_warp(&sh.p_full[1], turn[1] & 1, 48);
+                        if (!ok) break;
+                        ++turn[1];
+                        tc_fence_after();
+                        issue_pv(1, item, t == 0, last, true);
+                        if (more) issue_qk(1, item + 1, true, t + 2 == n_tiles);
+                    }
+                    item += more ? 2 : 1;
                 }
             }
+            if (!ok && lane == 0) sh.failed = 1;
         }
-        if (!ok && lane == 0) failed_s = 1;
     } else {
         // ------------------------------------------------------------------ softmax, one thread per row
-        const int stream = (warp - 2) >> 2;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MANY_REGISTERS));
+        const int stream = (warp - 4) >> 2;
         const int quarter = warp & 3;                     // the tensor-memory lanes this warp may touch
         const int r = quarter * 32 + lane;
-        const int my_node0 = node0 + (paired ? stream * p.tile_nodes : 0);
-        const int rows = min(p.tile_nodes, n - my_node0) * p.group;
-        const bool active = quarter * 32 < rows;          // (the warp) else its rows are nobody's
-        const bool mine = r < rows;
-        const int node = my_node0 + (mine ? r / p.group : 0), head = kvh * p.group + (mine ? r % p.group : 0);
-        const int pos = p.positions[token0 + node];
-        const int lo_r = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-        const uint32_t tmem = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(stream * STREAM_COLS);
-        float m_used = -INFINITY, l = 0.0f;
-        bool sees_odd = false, ok = true;
+        const uint32_t tmem_rows = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t tmem = tmem_rows + (uint32_t)(stream * STREAM_COLS);
         auto wait_all = [&](unsigned long long* bar, uint32_t parity, int code) {
             return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, p.error_flag, code)) != 0;
         };
-        // A tile that not every row sees alike holds a node, or a cached key in front of some node's window.  The latest position is at
-        // most length + n - 1.
-        const int window_end = p.window > 0 ? max(0, span.total - p.window) : 0;
-        int turn = 0, looked = 0;                         // the stream's tiles, and those of them that were looked through
-        for (int t = paired ? 0 : stream; t < n_tiles; t += dt, ++turn) {
-            const int kbase = (span.first + t) * BN;
-            const bool edge = kbase + BN > length || kbase < window_end;
-            lag_point();
-            ok = wait_all(&s_full[stream], turn & 1, 52);
-            if (!ok) break;
-            tc_fence_after();
-            unsigned seen[4];
-            if (edge) {
-#pragma unroll
-                for (int w = 0; w < 4; ++w) seen[w] = 0u;
-                if (mine) {
-                    const int j0 = kbase - length;        // the node at column 0, if any
-                    const int* const row = p.masks + (size_t)(token0 + node) * p.words;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int first = kbase + w * 32, j = j0 + w * 32;
-                        unsigned bits = bit_range(lo_r - first, length - first);             // cached keys
-                        if (j + 31 >= 0 && j < n) {
-                            // the 32 mask bits from bit j on (j may be negative)
-                            const int at = j >> 5;        // rounds down
-                            const unsigned low = at >= 0 && at < p.words ? (unsigned)row[at] : 0u, high = at + 1 >= 0 && at + 1 < p.words ? (unsigned)row[at + 1] : 0u;
-                            unsigned nodes = __funnelshift_r(low, high, (unsigned)(j & 31)) & bit_range(-j, n - j);
-                            if (p.window > 0 && lo_r > length) {
-                                // a window shorter than the tree is deep
-                                for (unsigned left = nodes; left; left &= left - 1) {
-                                    const int b = __ffs(left) - 1;
-                                    if (p.positions[token0 + j + b] < lo_r) nodes &= ~(1u << b);
+        bool ok = true;
+        int item0 = 0, turn = 0, shared_pieces = 0;       // the piece's first ring item; this stream's tiles; pieces whose rows the streams share
+        int looked[2] = {0, 0};                           // tiles looked through by this stream alone, by both
+        int results[2] = {0, 0};                          // accumulators finished, of each stream
+        while (ok && walk.next(p, stretch, lead)) {
+            const Sequence& s = walk.s;
+            const bool paired = walk.item.paired;
+            const int n_tiles = walk.n_tiles, kvh = walk.item.kvh, total = s.length + s.n, dt = paired ? 1 : 2;
+            const int my_node0 = walk.item.node0 + (paired ? stream * p.tile_nodes : 0);
+            const int rows = min(p.tile_nodes, s.n - my_node0) * p.group;
+            const bool active = quarter * 32 < rows;      // (the warp) else its rows are nobody's
+            const bool mine = r < rows;
+            const int node = my_node0 + (mine ? r / p.group : 0), head = kvh * p.group + (mine ? r % p.group : 0);
+            const int pos = p.positions[s.token0 + node];
+            const int lo_r = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+            float m_used = -INFINITY, l = 0.0f;
+            bool sees_odd = false;
+            // A tile that not every row sees alike holds a node, or a cached key in front of some node's window.  The latest position is at
+            // most length + n - 1.
+            const int window_end = p.window > 0 ? max(0, total - p.window) : 0;
+            bool first = true;
+            for (int t = paired ? 0 : stream; t < n_tiles; t += dt, ++turn, first = false) {
+                const int kbase = (s.first + walk.tile + t) * BN;
+                const bool edge = kbase + BN > s.length || kbase < window_end;
+                unsigned seen[4];
+                if (edge) {
+#pragma unroll 1
+                    for (int w = 0; w < 4; ++w) seen[w] = 0u;
+                    if (mine) {
+                        const int j0 = kbase - s.length;  // the node at column 0, if any
+                        const int* const row = p.masks + (size_t)(s.token0 + node) * p.words;
+#pragma unroll 1
+                        for (int w = 0; w < 4; ++w) {
+                            const int from = kbase + w * 32, j = j0 + w * 32;
+                            unsigned bits = bit_range(lo_r - from, s.length - from);             // cached keys
+                            if (j + 31 >= 0 && j < s.n) {
+                                // the 32 mask bits from bit j on (j may be negative)
+                                const int at = j >> 5;    // rounds down
+                                const unsigned low = at >= 0 && at < p.words ? (unsigned)row[at] : 0u, high = at + 1 >= 0 && at + 1 < p.words ? (unsigned)row[at + 1] : 0u;
+                                unsigned nodes = __funnelshift_r(low, high, (unsigned)(j & 31)) & bit_range(-j, s.n - j);
+                                if (p.window > 0 && lo_r > s.length) {
+                                    // a window shorter than the tree is deep
+                                    for (unsigned left = nodes; left; left &= left - 1) {
+                                        const int b = __ffs(left) - 1;
+                                        if (p.positions[s.token0 + j + b] < lo_r) nodes &= ~(1u << b);
+                                    }
                                 }
+                                bits |= nodes;
                             }
-                            bits |= nodes;
+                            seen[w] = bits;
                         }
-                        seen[w] = bits;
                     }
                 }
-            }
-            if (active) {
-                // Half a row at a time, read twice (for the maximum, for the exponentials): a whole one does not fit the registers that 10 warps leave a thread.
-                constexpr int HALF = BN / 2;
-                uint32_t sr[HALF];
-                auto half_row = [&](int h) {
-#pragma unroll
-                    for (int c = 0; c < HALF / 32; ++c) tmem_ld32(tmem + (uint32_t)(h * HALF + c * 32), sr + c * 32);
-                    tmem_wait_ld();
-                    if (edge) {
-#pragma unroll
-                        for (int c = 0; c < HALF; ++c)
-                            if (!((seen[h * 2 + (c >> 5)] >> (c & 31)) & 1u)) sr[c] = __float_as_uint(-INFINITY);
-                    }
-                };
-                half_row(0);
-                float top = row_max(sr);
-                half_row(1);
-                top = fmaxf(top, row_max(sr));
-                const float m_new = fmaxf(m_used, top * p.scale_log2);
-                const bool grow = m_new > m_used + RESCALE_STEP;      // also true for the first finite maximum
-                const float alpha = grow ? (m_used == -INFINITY ? 0.0f : fast_exp2(m_used - m_new)) : 1.0f;
-                if (turn > 0 && __any_sync(0xffffffffu, grow)) {
-#pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t o[32];
-                        tmem_ld32(tmem + (uint32_t)(O_COL + c * 32), o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tmem_st32(tmem + (uint32_t)(O_COL + c * 32), o);
-                    }
-                }
-                if (grow) { l *= alpha; m_used = m_new; }
-                const float shift = m_used == -INFINITY ? 0.0f : -m_used;
-                // the second half is still in the registers; the first half's P goes where the first half was, so it is the first to go back
-                uint32_t keep[HALF / 2];
-                l += row_exp2(sr, p.scale_log2, shift);
-#pragma unroll
-                for (int i = 0; i < HALF / 2; ++i) keep[i] = sr[i];
-                half_row(0);
-                l += row_exp2(sr, p.scale_log2, shift);
-                tmem_st32(tmem, sr);
-                tmem_st32(tmem + (uint32_t)(HALF / 2), keep);
-                tmem_wait_st();
-            }
-            if (edge) {
-                // the tile's value rows: warp q of a stream looks through and clears keys 32 q .. 32 q + 31 (where both streams read the tile, stream 0's warps do)
-                const int v_item = paired ? 1 + 2 * t : n_tiles == 1 ? 1 : 2 + t + min(t, n_tiles - 2);
-                const int owner = paired ? 0 : stream, key = kbase + r;
-                const bool nobodys = key >= span.total || key < span.lo;
-                const uint32_t vrow = ring_s + (v_item % SLOTS) * KV_BYTES + r * ROW_BYTES;
-                unsigned mark = 0u;
-                if (stream == owner) {
-                    ok = wait_all(&slot_full[v_item % SLOTS], (v_item / SLOTS) & 1, 53);
-                    if (!ok) break;
-                    bool odd = false;
-                    if (!nobodys) {
-                        uint32_t worst = 0u;              // an exponent of all ones is the largest there is
-#pragma unroll
-                        for (int i = 0; i < SPANS * 8; ++i) {
-                            uint32_t v[4];
-                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                                         : "r"(vrow + (i / 8) * (BN * ROW_BYTES) + (i % 8) * 16));
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) worst = __vmaxu2(worst, v[k] & 0x7f807f80u);
-                        }
-                        odd = (worst & 0x7f80u) == 0x7f80u || (worst >> 16) == 0x7f80u;
-                    }
-                    mark = __ballot_sync(0xffffffffu, odd);
-                    if (lane == 0) odd_s[owner][looked & 1][quarter] = mark;
-                    if (odd || nobodys) {
-#pragma unroll 1
-                        for (int i = 0; i < SPANS * 8; ++i)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vrow + (i / 8) * (BN * ROW_BYTES) + (i % 8) * 16), "r"(0u) : "memory");
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // for the tensor core
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&v_checked[owner]));
-                ok = wait_all(&v_checked[owner], looked & 1, 54);
+                lag_point();
+                ok = wait_all(&sh.s_full[stream], turn & 1, 49);
                 if (!ok) break;
+                tc_fence_after();
+                if (active) {
+                    // CHUNK scores at a time, read twice (for the maximum, for the exponentials)
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < BN / CHUNK; ++c) {
+                        uint32_t sr[CHUNK];
 #pragma unroll
-                for (int w = 0; w < 4; ++w) sees_odd |= (seen[w] & *(volatile unsigned*)&odd_s[owner][looked & 1][w]) != 0u;
-                ++looked;
+                        for (int i = 0; i < CHUNK / 32; ++i) tmem_ld32(tmem + (uint32_t)(c * CHUNK + i * 32), sr + i * 32);
+                        tmem_wait_ld();
+                        if (edge) {
+#pragma unroll
+                            for (int i = 0; i < CHUNK / 32; ++i) {
+                                const unsigned bits = seen[c * (CHUNK / 32) + i];
+#pragma unroll
+                                for (int k = 0; k < 32; ++k)
+                                    if (!((bits >> k) & 1u)) sr[i * 32 + k] = __float_as_uint(-INFINITY);
+                                tmem_st32(tmem + (uint32_t)(c * CHUNK + i * 32), sr + i * 32);
+                            }
+                        }
+                        top = fmaxf(top, row_max(sr));
+                    }
+                    if (edge) tmem_wait_st();
+                    const float m_new = fmaxf(m_used, top * p.scale_log2);
+                    const bool grow = m_new > m_used + RESCALE_STEP;      // also true for the first finite maximum
+                    const float alpha = grow ? (m_used == -INFINITY ? 0.0f : fast_exp2(m_used - m_new)) : 1.0f;
+                    if (!first && __any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(tmem + (uint32_t)(O_COL + c * 16), o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st16(tmem + (uint32_t)(O_COL + c * 16), o);
+                        }
+                    }
+                    if (grow) { l *= alpha; m_used = m_new; }
+                    const float shift = m_used == -INFINITY ? 0.0f : -m_used;
+                    // (P of a chunk goes where this chunk's or an earlier one's scores were)
+#pragma unroll 1
+                    for (int c = 0; c < BN / CHUNK; ++c) {
+                        uint32_t sr[CHUNK];
+#pragma unroll
+                        for (int i = 0; i < CHUNK / 32; ++i) tmem_ld32(tmem + (uint32_t)(c * CHUNK + i * 32), sr + i * 32);
+                        tmem_wait_ld();
+                        l += row_exp2(sr, p.scale_log2, shift);
+                        if constexpr (CHUNK == 64) tmem_st32(tmem + (uint32_t)(c * 32), sr);
+                        else tmem_st16(tmem + (uint32_t)(c * 16), sr);
+                    }
+                    tmem_wait_st();
+                }
+                if (edge) {
+                    // the tile's value rows: warp q of a stream looks through and clears keys 32 q .. 32 q + 31 (where both streams read the tile, stream 0's warps do)
+                    const int v_item = item0 + (paired ? 1 + 2 * t : n_tiles == 1 ? 1 : 2 + t + min(t, n_tiles - 2));
+                    const int which = paired ? 2 : stream, buffer = looked[paired] & 1, key = kbase + r;
+                    const bool nobodys = key >= total || key < s.lo;
+                    const uint32_t vrow = ring_s + (v_item % SLOTS) * KV_BYTES + r * ROW_BYTES;
+                    if (!paired || stream == 0) {
+                        ok = wait_all(&sh.slot_full[v_item % SLOTS], (v_item / SLOTS) & 1, 50);
+                        if (!ok) break;
+                        bool odd = false;
+                        if (!nobodys) {
+                            uint32_t worst = 0u;          // an exponent of all ones is the largest there is
+#pragma unroll 4
+                            for (int i = 0; i < SPANS * 8; ++i) {
+                                uint32_t v[4];
+                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                                             : "r"(vrow + (i / 8) * (BN * ROW_BYTES) + (i % 8) * 16));
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) worst = __vmaxu2(worst, v[k] & 0x7f807f80u);
+                            }
+                            odd = (worst & 0x7f80u) == 0x7f80u || (worst >> 16) == 0x7f80u;
+                        }
+                        const unsigned mark = __ballot_sync(0xffffffffu, odd);
+                        if (lane == 0) sh.odd[which][buffer][quarter] = mark;
+                        if (odd || nobodys) {
+#pragma unroll 1
+                            for (int i = 0; i < SPANS * 8; ++i)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vrow + (i / 8) * (BN * ROW_BYTES) + (i % 8) * 16), "r"(0u) : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // for the tensor core
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sh.v_checked[which]));
+                    ok = wait_all(&sh.v_checked[which], buffer, 51);
+                    if (!ok) break;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) sees_odd |= (seen[w] & *(volatile unsigned*)&sh.odd[which][buffer][w]) != 0u;
+                    ++looked[paired];
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[stream]));
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&p_full[stream]));
-        }
-        // ---- the rows' results.  Streams that share the rows meet: each takes half of the columns of both accumulators.
-        float weight[2] = {0.0f, 0.0f}, m_all = m_used, l_all = sees_odd ? NAN : l;
-        weight[stream] = 1.0f;
-        if (!paired) {
-            norm_s[stream * BM + r] = make_float2(m_used, l_all);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&norms_there));
-            ok = wait_all(&norms_there, 0, 55) && ok;
-            if (ok) {
-                const float2 a = norm_s[r], b = norm_s[BM + r];
+            if (!ok) break;
+            item0 += 2 * n_tiles;
+            // ---- the rows' results.  Streams that share the rows meet: each takes half of the columns of both accumulators.
+            float weight[2] = {0.0f, 0.0f}, m_all = m_used, l_all = sees_odd ? NAN : l;
+            weight[stream] = 1.0f;
+            if (!paired) {
+                sh.norm[stream * BM + r] = make_float2(m_used, l_all);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.norms_there));
+                ok = wait_all(&sh.norms_there, shared_pieces & 1, 52);
+                if (!ok) break;
+                const float2 a = sh.norm[r], b = sh.norm[BM + r];
                 m_all = fmaxf(a.x, b.x);
                 weight[0] = a.x == -INFINITY ? 0.0f : fast_exp2(a.x - m_all);
                 weight[1] = b.x == -INFINITY ? 0.0f : fast_exp2(b.x - m_all);
                 l_all = a.y * weight[0] + b.y * weight[1];
                 if (isnan(a.y) || isnan(b.y)) l_all = NAN;
             }
-        }
-        const bool has[2] = {paired ? stream == 0 && n_tiles > 0 : n_tiles > 0, paired ? stream == 1 && n_tiles > 0 : n_tiles > 1};
-        for (int s = 0; s < 2; ++s)
-            if (ok && has[s]) ok = wait_all(&o_full[s], 0, 56);
-        if (ok && active) {
-            tc_fence_after();
-            const float inv = p.shares > 1 ? 1.0f : l_all > 0.0f ? 1.0f / l_all : isnan(l_all) ? NAN : 0.0f;
-            const float w0 = weight[0] * inv, w1 = weight[1] * inv;
-            const size_t row = (size_t)(token0 + node) * p.heads + head;
-            const int c_begin = paired ? 0 : stream * (D / 64), c_end = paired ? D / 32 : c_begin + D / 64;
-            const uint32_t tmem_rows = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)O_COL;
-#pragma unroll 1
-            for (int c = c_begin; c < c_end; ++c) {
-                float o[32];
+            // whose accumulators this warp reads, and which there are
+            const bool made[2] = {true, paired || n_tiles > 1}, has[2] = {!paired || stream == 0, paired ? stream == 1 : n_tiles > 1};
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = 0.0f;
-                uint32_t x[32];
-                if (has[0]) {
-                    tmem_ld32(tmem_rows + (uint32_t)(c * 32), x);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = w0 == 0.0f ? 0.0f : __uint_as_float(x[i]) * w0;
-                }
-                if (has[1]) {
-                    tmem_ld32(tmem_rows + (uint32_t)(STREAM_COLS + c * 32), x);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = w1 == 0.0f ? o[i] : fmaf(__uint_as_float(x[i]), w1, o[i]);
-                }
-                if (mine && p.shares > 1) {
-                    float4* const to = reinterpret_cast<float4*>(p.part_out + ((size_t)share * p.tokens * p.heads + row) * D + c * 32);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) to[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                } else if (mine) {
-                    uint4* const to = reinterpret_cast<uint4*>(p.out + row * D + c * 32);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        to[i] = make_uint4(pack_bf16(o[8 * i], o[8 * i + 1]), pack_bf16(o[8 * i + 2], o[8 * i + 3]), pack_bf16(o[8 * i + 4], o[8 * i + 5]),
-                                           pack_bf16(o[8 * i + 6], o[8 * i + 7]));
-                }
-                __syncwarp();
+            for (int i = 0; i < 2; ++i) {
+                if (ok && has[i]) ok = wait_all(&sh.o_full[i], results[i] & 1, 53);
+                results[i] += made[i] ? 1 : 0;
             }
-            if (mine && p.shares > 1 && (paired || stream == 0)) p.part_norm[(size_t)share * p.tokens * p.heads + row] = make_float2(m_all, l_all);
+            if (!ok) break;
+            tc_fence_after();
+            if (active) {
+                const bool whole = walk.parts == 1;
+                const float inv = !whole ? 1.0f : l_all > 0.0f ? 1.0f / l_all : isnan(l_all) ? NAN : 0.0f;
+                const float w0 = weight[0] * inv, w1 = weight[1] * inv;
+                const size_t row = (size_t)(s.token0 + node) * p.heads + head;
+                const size_t part = ((size_t)blockIdx.x * 2 + (walk.part == 0 ? 1 : 0)) * 2 + (paired ? stream : 0);
+                const int c_begin = paired ? 0 : stream * (D / 32), c_end = paired ? D / 16 : c_begin + D / 32;
+#pragma unroll 1
+                for (int c = c_begin; c < c_end; ++c) {
+                    float o[16];
+                    uint32_t x[2][16];
+                    if (has[0]) tmem_ld16(tmem_rows + (uint32_t)(O_COL + c * 16), x[0]);
+                    if (has[1]) tmem_ld16(tmem_rows + (uint32_t)(STREAM_COLS + O_COL + c * 16), x[1]);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        o[i] = has[0] && w0 != 0.0f ? __uint_as_float(x[0][i]) * w0 : 0.0f;
+                        if (has[1] && w1 != 0.0f) o[i] = fmaf(__uint_as_float(x[1][i]), w1, o[i]);
+                    }
+                    if (mine && !whole) {
+                        // a column's rows lie together: a warp's store is one line (rows beside one another would be 32, and took 4 us of 50)
+                        float* const to = p.part_out + (part * D + c * 16) * BM + r;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) to[i * BM] = o[i];
+                    } else if (mine) {
+                        uint4* const to = reinterpret_cast<uint4*>(p.out + row * D + c * 16);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            to[i] = make_uint4(pack_bf16(o[8 * i], o[8 * i + 1]), pack_bf16(o[8 * i + 2], o[8 * i + 3]), pack_bf16(o[8 * i + 4], o[8 * i + 5]),
+                                               pack_bf16(o[8 * i + 6], o[8 * i + 7]));
+                    }
+                    __syncwarp();
+                }
+                if (mine && !whole && (paired || stream == 0)) p.part_norm[part * BM + r] = make_float2(m_all, l_all);
+            }
+            tc_fence_before();                            // the accumulators were read before what the next piece's first P releases
+            if (!paired) {
+                // the other stream's accumulator too: nobody hands over a new P before everybody has read
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&sh.o_read));
+                ok = wait_all(&sh.o_read, shared_pieces & 1, 54);
+                ++shared_pieces;
+            }
         }
-        if (!ok) failed_s = 1;
+        if (!ok) sh.failed = 1;
     }
 
     tc_fence_before();
     __syncthreads();
-    if (failed_s && warp == 0 && lane == 0) {
+    if (sh.failed && warp == 0 && lane == 0) {
         // give the copies in flight a bounded chance to land before the CTA's memory goes away
-        mbar_wait(smem_u32(&q_full), 0, nullptr, 0);
-        for (int i = max(0, issued - SLOTS); i < issued; ++i) mbar_wait(smem_u32(&slot_full[i % SLOTS]), (i / SLOTS) & 1, nullptr, 0);
+        if (sh.pieces > 0) mbar_wait(smem_u32(&sh.q_full), (sh.pieces - 1) & 1, nullptr, 0);
+        for (int i = max(0, sh.issued - SLOTS); i < sh.issued; ++i) mbar_wait(smem_u32(&sh.slot_full[i % SLOTS]), (i / SLOTS) & 1, nullptr, 0);
     }
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)TMEM_COLS) : "memory");
     }
 }
 
-// The shares of a row in their order: a quarter warp a row, four columns of a span a lane.
-constexpr int JOIN_THREADS = 128;
+// The parts of the rows of items that lie in several CTAs, in a fixed order.  A CTA takes 32 rows of a row tile, a lane a row.  Its eight warps take
+//     SPREAD:  the parts in turn, all for the same 16 columns, and meet in shared memory: a call of few rows has many parts, and waits for one chain
+//              of loads, not for the bandwidth
+//     else:    an eighth of the columns each, all parts: a call of many rows has few parts a row
+constexpr int JOIN_THREADS = 256, JOIN_ROWS = 32, JOIN_WARPS = JOIN_THREADS / 32;
+template <bool SPREAD>
 __global__ void __launch_bounds__(JOIN_THREADS) draft_join_tc_kernel(TcParams p) {
     pdl_prologue();
-    constexpr int LANES = D / 4, ROWS = JOIN_THREADS / LANES;
-    const int seq = blockIdx.y, start = p.starts[seq], n = p.starts[seq + 1] - start, length = p.lengths[seq];
-    const int at = blockIdx.x * ROWS + threadIdx.x / LANES, c = (threadIdx.x % LANES) * 4;
-    if (at >= min(n, p.max_nodes) * p.heads) return;
-    const size_t row = (size_t)start * p.heads + at, all_rows = (size_t)p.tokens * p.heads;
-    const int lo = p.window > 0 ? max(0, length - p.window + 1) : 0, per = p.share / BN;
-    const int shares = min(p.shares, ((length + n + BN - 1) / BN - lo / BN + per - 1) / per);
-    float top = -INFINITY;
-    for (int s = 0; s < shares; ++s) top = fmaxf(top, p.part_norm[s * all_rows + row].x);
-    float4 acc = make_float4(0, 0, 0, 0);
-    float sum = 0.0f;
+    constexpr int COLS = SPREAD ? 16 : D / JOIN_WARPS, CHUNKS = SPREAD ? D / COLS : 1;
+    __shared__ float acc_s[SPREAD ? JOIN_WARPS : 1][COLS][JOIN_ROWS];
+    __shared__ float2 norm_s[SPREAD ? JOIN_WARPS : 1][JOIN_ROWS];
+    const int seq = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int stretch = p.line[0], lead = p.line[1], base = p.line[2 + seq];
+    const Sequence s = sequence_at(p, seq);
+    int at = blockIdx.x;
+    const int col0 = SPREAD ? at % CHUNKS * COLS : warp * COLS;
+    at /= CHUNKS;
+    const int block = at % (BM / JOIN_ROWS);
+    at /= BM / JOIN_ROWS;
+    const int tile = at % p.row_tiles, kvh = at / p.row_tiles;
+    if (tile >= s.row_tiles) return;
+    const int node0 = tile * p.tile_nodes, rows = min(p.tile_nodes, s.n - node0) * p.group - block * JOIN_ROWS;      // from this block's first on
+    if (rows <= 0) return;
+    const Item item = item_of(p, s, base, lead, kvh, tile >> 1);
+    const int first = item.begin / stretch, parts = (item.end - 1) / stretch - first + 1;
+    if (parts == 1) return;                               // written whole
+    const bool mine = lane < rows;
+    float top = -INFINITY, sum = 0.0f, acc[COLS] = {};
 #pragma unroll 4
-    for (int s = 0; s < shares; ++s) {
-        const float2 norm = p.part_norm[s * all_rows + row];
-        const float4 o = *reinterpret_cast<const float4*>(p.part_out + (s * all_rows + row) * D + c);
-        const float w = norm.x == -INFINITY ? 0.0f : exp2f(norm.x - top);
-        if (norm.x == -INFINITY && !isnan(norm.y)) continue;
-        sum += isnan(norm.y) ? NAN : norm.y * w;
-        acc = make_float4(fmaf(w, o.x, acc.x), fmaf(w, o.y, acc.y), fmaf(w, o.z, acc.z), fmaf(w, o.w, acc.w));
+    for (int k = SPREAD ? warp : 0; k < parts; k += SPREAD ? JOIN_WARPS : 1) {
+        // part k lies with CTA first + k: the first part is of the item that its stretch ends in, the others of the one that it begins in; a part
+        // may be no tile's
+        const bool there = mine && tile_of(item, min((first + k + 1) * stretch, item.end)) > tile_of(item, max((first + k) * stretch, item.begin));
+        const size_t slot = ((size_t)(first + k) * 2 + (k == 0 ? 1 : 0)) * 2 + (tile & 1);
+        const float2 norm = there ? p.part_norm[slot * BM + block * JOIN_ROWS + lane] : make_float2(-INFINITY, 0.0f);
+        const float* const o = p.part_out + (slot * D + col0) * BM + block * JOIN_ROWS + lane;
+        float v[COLS];
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) v[i] = there ? o[i * BM] : 0.0f;
+        const float m = fmaxf(top, norm.x);
+        const float keep = top == -INFINITY ? 0.0f : exp2f(top - m), w = norm.x == -INFINITY ? 0.0f : exp2f(norm.x - m);
+        sum = sum * keep + (norm.x == -INFINITY && !isnan(norm.y) ? 0.0f : norm.y * w);
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) acc[i] = w == 0.0f ? acc[i] * keep : fmaf(w, v[i], acc[i] * keep);
+        top = m;
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : isnan(sum) ? NAN : 0.0f;
-    *reinterpret_cast<uint2*>(p.out + row * D + c) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    auto row_of = [&](int r) {
+        const int in_tile = block * JOIN_ROWS + r;
+        return (size_t)(s.token0 + node0 + in_tile / p.group) * p.heads + kvh * p.group + in_tile % p.group;
+    };
+    auto inverse = [](float sum) { return sum > 0.0f ? 1.0f / sum : isnan(sum) ? NAN : 0.0f; };
+    if constexpr (!SPREAD) {
+        if (!mine) return;
+        const float inv = inverse(sum);
+        uint4* const to = reinterpret_cast<uint4*>(p.out + row_of(lane) * D + col0);
+#pragma unroll
+        for (int i = 0; i < COLS / 8; ++i)
+            to[i] = make_uint4(pack_bf16(acc[8 * i] * inv, acc[8 * i + 1] * inv), pack_bf16(acc[8 * i + 2] * inv, acc[8 * i + 3] * inv),
+                               pack_bf16(acc[8 * i + 4] * inv, acc[8 * i + 5] * inv), pack_bf16(acc[8 * i + 6] * inv, acc[8 * i + 7] * inv));
+    } else {
+        norm_s[warp][lane] = make_float2(top, sum);
+#pragma unroll
+        for (int i = 0; i < COLS; ++i) acc_s[warp][i][lane] = acc[i];
+        __syncthreads();
+        // a thread two columns of a row
+        const int r = threadIdx.x / (COLS / 2), c = threadIdx.x % (COLS / 2) * 2;
+        if (r >= rows) return;
+        top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < JOIN_WARPS; ++w) top = fmaxf(top, norm_s[w][r].x);
+        float a = 0.0f, b = 0.0f;
+        sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < JOIN_WARPS; ++w) {
+            const float2 norm = norm_s[w][r];
+            const float f = norm.x == -INFINITY ? 0.0f : exp2f(norm.x - top);
+            sum += isnan(norm.y) ? NAN : norm.y * f;
+            a = f == 0.0f ? a : fmaf(f, acc_s[w][c][r], a);
+            b = f == 0.0f ? b : fmaf(f, acc_s[w][c + 1][r], b);
+        }
+        const float inv = inverse(sum);
+        *reinterpret_cast<uint32_t*>(p.out + row_of(r) * D + col0 + c) = pack_bf16(a * inv, b * inv);
+    }
 }
 
 // --------------------------------------------------------------------------------- host side
@@ -723,10 +985,11 @@ int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
 
 }  // namespace
 
-// q and out [T, NH * D] bf16, pages [num_pages, 2, NKV, page_size, D].  scratch: shares > 1: [shares, T * NH, D] fp32, then [shares, T * NH] float2.
+// q and out [T, NH * D] bf16, pages [num_pages, 2, NKV, page_size, D].  `ctas` CTAs take `stretch` units or more each; scratch, with more than one:
+// [ctas, 2, 2, D, 128] fp32, [ctas, 2, 2, 128] float2, [2 + sequences] int.
 MLB_EXPORT int mlb_draft_attention_tc(const void* q, const void* pages, void* out, const int* starts, const int* lengths, const int* positions, const int* masks,
                                       int words, const int* table, int max_blocks, int num_pages, int page_size, int tokens, int sequences, int max_nodes,
-                                      int heads, int kv_heads, float scale, int window, int share, int shares, void* scratch, int* error_flag,
+                                      int heads, int kv_heads, float scale, int window, int stretch, int ctas, void* scratch, int* error_flag,
                                       cudaStream_t stream) {
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || heads / kv_heads > BM)
         return fail(MLB_UNSUPPORTED_SIZE, "draft_attention_tc: heads %d/%d", heads, kv_heads);
@@ -736,13 +999,16 @@ MLB_EXPORT int mlb_draft_attention_tc(const void* q, const void* pages, void* ou
         return fail(MLB_UNSUPPORTED_SIZE, "draft_attention_tc: page_size %d must be a multiple of 8 that divides %d", page_size, BN);
     if (!(scale > 0.0f)) return fail(MLB_UNSUPPORTED_SIZE, "draft_attention_tc: the softmax scale must be positive");
     if (num_pages <= 0 || max_blocks <= 0 || tokens < 0 || sequences < 0 || window < 0) return fail(MLB_INVALID_ARGUMENT, "draft_attention_tc: bad sizes");
-    if (share <= 0 || share % BN != 0 || shares <= 0 || (shares > 1 && !scratch)) return fail(MLB_INVALID_ARGUMENT, "draft_attention_tc: bad shares");
+    if (stretch <= 0 || ctas <= 0 || (ctas > 1 && !scratch)) return fail(MLB_INVALID_ARGUMENT, "draft_attention_tc: bad cut");
     if (((uintptr_t)q & 15) || ((uintptr_t)out & 15) || ((uintptr_t)pages & 15) || ((uintptr_t)scratch & 15))
         return fail(MLB_UNSUPPORTED_SIZE, "draft_attention_tc: q, out, the pages and the scratch must be 16-byte aligned");
     const long long kv_rows = (long long)num_pages * 2 * kv_heads * page_size;
     if (kv_rows >= (1ll << 31)) return fail(MLB_UNSUPPORTED_SIZE, "draft_attention_tc: the cache has too many rows (%lld)", kv_rows);
-    const int group = heads / kv_heads, tile_nodes = BM / group, pairs = (max_nodes + 2 * tile_nodes - 1) / (2 * tile_nodes);
-    if (sequences > 65535 || pairs * kv_heads > 65535) return fail(MLB_UNSUPPORTED_SIZE, "draft_attention_tc: too many sequences or rows");
+    const int group = heads / kv_heads, tile_nodes = BM / group;
+    // every count of units fits 31 bits: a sequence's tiles are at most the table's
+    const long long most_tiles = ((long long)max_blocks * page_size + BN - 1) / BN + 1;
+    if (most_tiles * ((max_nodes + tile_nodes - 1) / tile_nodes) * (1 + MOST_LEAD) * kv_heads * (sequences > 0 ? sequences : 1) >= (1ll << 30) || sequences > 65535)
+        return fail(MLB_UNSUPPORTED_SIZE, "draft_attention_tc: too much work for a call");
     if (tokens == 0 || sequences == 0) return MLB_OK;
 
     CUtensorMap map_q, map_kv;
@@ -759,9 +1025,12 @@ MLB_EXPORT int mlb_draft_attention_tc(const void* q, const void* pages, void* ou
         if (status != MLB_OK) return status;
     }
     TcParams p{(__nv_bfloat16*)out, starts, lengths, positions, masks, table, words, max_blocks, num_pages, page_size, BN / page_size, heads, kv_heads, group,
-               tile_nodes, pairs, window, max_nodes, share, shares, tokens, scale * LOG2E, nullptr, nullptr, error_flag};
-    p.part_out = (float*)scratch;
-    p.part_norm = (float2*)((float*)scratch + (size_t)shares * tokens * heads * D);
+               tile_nodes, (max_nodes + tile_nodes - 1) / tile_nodes, window, max_nodes, stretch, ctas, sequences, tokens, scale * LOG2E, nullptr, nullptr, nullptr, error_flag};
+    if (ctas > 1) {
+        p.part_out = (float*)scratch;
+        p.part_norm = (float2*)(p.part_out + (size_t)ctas * 4 * BM * D);
+        p.line = (int*)(p.part_norm + (size_t)ctas * 4 * BM);
+    }
     static bool configured_on[MAX_DEVICES] = {false};         // the attribute belongs to the device
     bool& configured = configured_on[device_index()];
     if (!configured) {
@@ -769,10 +1038,11 @@ MLB_EXPORT int mlb_draft_attention_tc(const void* q, const void* pages, void* ou
             return check_launch("draft_attention_tc: shared memory");
         configured = true;
     }
-    launch_kernel(draft_attention_tc_kernel, dim3(shares, pairs * kv_heads, sequences), THREADS, SMEM_BYTES, stream, map_q, map_kv, p);
+    launch_kernel(draft_attention_tc_kernel, ctas, THREADS, SMEM_BYTES, stream, map_q, map_kv, p);
     const int status = check_launch("draft_attention_tc");
-    if (status != MLB_OK || shares == 1) return status;
-    constexpr int rows = JOIN_THREADS / (D / 4);
-    launch_kernel(draft_join_tc_kernel, dim3((max_nodes * heads + rows - 1) / rows, sequences), JOIN_THREADS, 0, stream, p);
+    if (status != MLB_OK || ctas == 1) return status;
+    const int blocks = kv_heads * p.row_tiles * (BM / JOIN_ROWS);
+    if ((long long)blocks * sequences <= sm_count()) launch_kernel(draft_join_tc_kernel<true>, dim3(blocks * (D / 16), sequences), JOIN_THREADS, 0, stream, p);
+    else launch_kernel(draft_join_tc_kernel<false>, dim3(blocks, sequences), JOIN_THREADS, 0, stream, p);
     return check_launch("draft_join_tc");
 }

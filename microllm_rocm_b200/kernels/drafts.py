@@ -22,6 +22,7 @@ MAX_NODES = 256             # csrc/drafts.cu: nodes of a sequence
 ROWS, KEYS = 16, 32         # csrc/drafts.cu: rows (node, head of a group) and keys a CTA works on at a time
 SHARE_KEYS = 64             # keys below which a share is not cut further
 TC_HEAD_DIMS, TC_KEYS, TC_ROWS = (64, 128), 128, 128        # csrc/drafts_tc.cu: keys a tile, rows of a stream (a CTA has two)
+TC_STRETCH = 2              # units (row tile x key tile) a CTA takes at least: a turn of both streams
 
 ops.register_signatures("drafts.cu", {
     "mlb_draft_masks": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
@@ -84,6 +85,11 @@ def _shares(ctas: int, keys: int, sms: int):
     return share, -(-keys // share)
 
 
+def _ctas(heads: int, row_tiles: int, key_tiles: int, sms: int) -> int:
+    """CTAs of the tensor-core kernel: one a multiprocessor, as long as each finds TC_STRETCH units of heads x row tiles x key tiles."""
+    return max(1, min(sms, -(-heads * row_tiles * key_tiles // TC_STRETCH)))
+
+
 def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor,
                     masks: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
                     window: Optional[int] = None, *, max_nodes: int, max_length: int, error_flag: Optional[torch.Tensor] = None) -> None:
@@ -124,15 +130,12 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     group = num_heads // num_kv_heads
     if q.dtype == torch.bfloat16 and tc_supported(head_dim, page_size, group, scale) and not (q.data_ptr() | pages.data_ptr() | out.data_ptr()) & 15:
         keys = min(max_length, window + max_nodes + TC_KEYS) if window else max_length
-        tiles, pairs = -(-keys // TC_KEYS), -(-max_nodes // (2 * (TC_ROWS // group)))
-        shares = max(1, min(tiles, sm_count(q.device) // max(1, sequences * num_kv_heads * pairs)))
-        per = -(-tiles // shares)
-        shares = -(-tiles // per)
-        scratch = ops.scratch(shares * T * num_heads * (head_dim + 2) * 4, q.device, "draft_attention") if shares > 1 else None
+        ctas = _ctas(sequences * num_kv_heads, -(-max_nodes // (TC_ROWS // group)), -(-keys // TC_KEYS), sm_count(q.device))
+        scratch = ops.scratch(ctas * 4 * TC_ROWS * (head_dim + 2) * 4 + 8 + 4 * sequences, q.device, "draft_attention") if ctas > 1 else None
         L = ops.lib("drafts_tc.cu", {"HEAD_DIM": head_dim})
         build.check(L, L.mlb_draft_attention_tc(q.data_ptr(), pages.data_ptr(), out.data_ptr(), starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
                                                 masks.data_ptr(), words, block_table.data_ptr(), block_table.shape[1], num_pages, page_size, T, sequences,
-                                                int(max_nodes), num_heads, num_kv_heads, float(scale), int(window or 0), per * TC_KEYS, shares, ops._ptr(scratch),
+                                                int(max_nodes), num_heads, num_kv_heads, float(scale), int(window or 0), TC_STRETCH, ctas, ops._ptr(scratch),
                                                 ops._ptr(error_flag), ops._stream()))
         return
     keys = min(max_length, window + max_nodes + KEYS) if window else max_length

@@ -157,7 +157,7 @@ def lagged_latent_sources():
 
 def lagged_draft_sources():
     """And of the attention of drafted trees: both copying and issuing warps, and a softmax warp of each stream."""
-    return [("drafts_tc.cu", {"HEAD_DIM": 128, "MLB_LAG_WARP": w}) for w in (0, 1, 3, 8)]
+    return [("drafts_tc.cu", {"HEAD_DIM": 128, "MLB_LAG_WARP": w}) for w in (0, 1, 5, 10)]
 
 
 def lib(source: str, defines=None) -> ctypes.CDLL:

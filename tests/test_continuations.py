@@ -140,6 +140,10 @@ def test_shares_cover_the_keys(ctas, keys):
     assert ctas * shares <= max(2 * 148, ctas)
 
 
+def test_tensor_core_attention_takes_a_cta_a_multiprocessor_at_most():
+    assert [drafts._ctas(*x, 148) for x in ((1, 1, 1), (2, 2, 17), (64, 4, 17), (1, 1, 2))] == [1, 34, 148, 1]
+
+
 def test_scratch_on_the_second_stream_is_the_steps(monkeypatch):
     monkeypatch.setattr(ops, "second_stream", lambda: (7, None))
     with pytest.raises(KernelError, match="second stream"):
