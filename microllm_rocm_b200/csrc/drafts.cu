@@ -86,22 +86,38 @@ struct DraftParams {
 // the first key that any node of a sequence may see
 __device__ __forceinline__ int first_key(int length, int window) { return window > 0 ? max(0, length - window + 1) : 0; }
 
-// PIECES: rows of the cache and of q are read in pieces of four elements.  COLS columns and RPT rows a thread in the second product.
+// PIECES: the cache's rows are copied in pieces of 16 bytes, asynchronously, a tile ahead of the one that is worked on; else element by element.
+// Keys and values lie in shared memory in the cache's type.  COLS columns and RPT rows a thread in the second product.
+template <typename T> __device__ __forceinline__ void unpack(const uint4& x, float (&v)[16 / sizeof(T)]) {
+    const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(w[i]);
+        else { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+}
+
+template <typename T, int DMAX> constexpr int attention_smem() {
+    return ROWS * DMAX * 4 + 2 * KEYS * (2 * DMAX + 16 / (int)sizeof(T)) * (int)sizeof(T);
+}
+
 template <typename T, int DMAX, bool PIECES>
 __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p) {
     pdl_prologue();
     constexpr int COLS = DMAX > 128 ? 2 : 1;
     constexpr int RPT = DMAX >= 128 ? ROWS : DMAX / 8;         // 32: 4, 64: 8
-    constexpr int PITCH = DMAX + 4;
-    extern __shared__ float smem[];
-    float* const q_s = smem;                                   // [ROWS][DMAX]
-    float* const k_s = q_s + ROWS * DMAX;                      // [KEYS][PITCH]
-    float* const v_s = k_s + KEYS * PITCH;                     // [KEYS][DMAX]
+    constexpr int EPP = 16 / sizeof(T);                        // elements a piece
+    constexpr int PITCH = DMAX + EPP;                          // of a key row: neighbouring lanes' pieces in different banks
+    constexpr int P = DMAX / EPP, MINE = KEYS * P / THREADS > 0 ? KEYS * P / THREADS : 1;      // pieces of a row, and a thread's of a tile
+    static_assert(KEYS * P % THREADS == 0, "whole rounds of pieces");
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* const q_s = reinterpret_cast<float*>(smem);         // [ROWS][DMAX]
+    T* const k_s = reinterpret_cast<T*>(q_s + ROWS * DMAX);    // [2][KEYS][PITCH]
+    T* const v_s = k_s + 2 * KEYS * PITCH;                     // [2][KEYS][DMAX]
     __shared__ __align__(16) float p_s[ROWS][KEYS];
     __shared__ float alpha_s[ROWS], sum_s[ROWS], max_s[ROWS];
     __shared__ unsigned mask_s[ROWS][MAX_WORDS];
-    __shared__ int pos_s[ROWS], key_pos_s[KEYS];
-    __shared__ long long key_at[KEYS];
+    __shared__ int pos_s[ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int share = blockIdx.x, seq = blockIdx.z;
     const int kvh = blockIdx.y / p.row_tiles, row0 = (blockIdx.y % p.row_tiles) * ROWS;
@@ -117,6 +133,40 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
     const int key_end = share == p.shares - 1 ? total : min(total, key_begin + p.share);
     if (share > 0 && key_begin >= total) return;
 
+    const size_t plane = (size_t)p.page_size * D, page_stride = 2 * plane * p.kv_heads, v_offset = plane * p.kv_heads;
+    const int* const table = p.table + (size_t)seq * p.max_blocks;
+    // where a key's row begins in the pool; -1: no row may see it, or it has no page
+    auto place_of = [&](int key) -> long long {
+        if (key < lo || key >= key_end) return -1;
+        const int block = key / p.page_size;
+        const int page = block < p.max_blocks ? table[block] : -1;
+        if (page < 0 || page >= p.num_pages) {
+            if (p.error_flag) atomicExch(p.error_flag, 2);
+            return -1;
+        }
+        return (long long)((size_t)page * page_stride + (size_t)kvh * plane + (size_t)(key % p.page_size) * D);
+    };
+    auto ask = [&](int base, int buffer) {                     // the pieces of a tile's keys and values
+        long long at[MINE];
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) at[i] = place_of(base + (tid + i * THREADS) / P);
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int e = tid + i * THREADS, key = e / P, c = e % P * EPP;
+            const bool there = at[i] >= 0 && c < D;
+            const T* const from = (const T*)p.pages + (there ? at[i] + c : 0);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(k_s + (buffer * KEYS + key) * PITCH + c)), "l"(from),
+                         "r"(there ? 16 : 0) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(v_s + (buffer * KEYS + key) * DMAX + c)), "l"(from + (there ? v_offset : 0)),
+                         "r"(there ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // the position of the lane's key; -1: not there
+    auto position_of = [&](int base) { return place_of(base + lane) < 0 ? -1 : base + lane < length ? base + lane : p.positions[start + base + lane - length]; };
+
+    if (PIECES) ask(key_begin, 0);
+    int where = position_of(key_begin);
     for (int e = tid; e < ROWS * DMAX; e += THREADS) {
         const int r = e / DMAX, c = e % DMAX;
         float v = 0.0f;
@@ -142,77 +192,57 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
     float m[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
-    const size_t plane = (size_t)p.page_size * D, page_stride = 2 * plane * p.kv_heads, v_offset = plane * p.kv_heads;
-    const int* const table = p.table + (size_t)seq * p.max_blocks;
 
-    for (int base = key_begin; base < key_end; base += KEYS) {
-        __syncthreads();                                       // the last tile's values were read
-        if (tid < KEYS) {
-            const int key = base + tid;
-            long long at = -1;
-            int where = -1;
-            if (key >= lo && key < key_end) {
-                const int block = key / p.page_size;
-                const int page = block < p.max_blocks ? table[block] : -1;
-                if (page < 0 || page >= p.num_pages) {
-                    if (p.error_flag) atomicExch(p.error_flag, 2);
-                } else {
-                    at = (long long)((size_t)page * page_stride + (size_t)kvh * plane + (size_t)(key % p.page_size) * D);
-                    where = key < length ? key : p.positions[start + key - length];
-                }
-            }
-            key_at[tid] = at;
-            key_pos_s[tid] = where;
-        }
-        __syncthreads();
+    int buffer = 0;
+    for (int base = key_begin; base < key_end; base += KEYS, buffer ^= 1) {
+        const bool more = base + KEYS < key_end;
+        const T* const k_t = k_s + buffer * KEYS * PITCH;
+        const T* const v_t = v_s + buffer * KEYS * DMAX;
         bool odd = false;                                      // a value that is not finite: it may not meet the zero weight of a row that does not see it
+        int where_next = -1;
         if (PIECES) {
-            constexpr int P = DMAX / 4;
-            for (int e = tid; e < KEYS * P; e += THREADS) {
-                const int key = e / P, c = (e % P) * 4;
-                const long long at = key_at[key];
-                float4 k4 = make_float4(0, 0, 0, 0), v4 = k4;
-                if (at >= 0 && c < D) {
-                    const T* const k = (const T*)p.pages + at + c;
-                    const T* const v = k + v_offset;
-                    if constexpr (sizeof(T) == 4) {
-                        k4 = *reinterpret_cast<const float4*>(k);
-                        v4 = *reinterpret_cast<const float4*>(v);
-                    } else {
-                        const uint2 a = *reinterpret_cast<const uint2*>(k), b = *reinterpret_cast<const uint2*>(v);
-                        k4 = make_float4(__uint_as_float(a.x << 16), __uint_as_float(a.x & 0xffff0000u), __uint_as_float(a.y << 16), __uint_as_float(a.y & 0xffff0000u));
-                        v4 = make_float4(__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u), __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u));
-                    }
-                }
-                *reinterpret_cast<float4*>(k_s + key * PITCH + c) = k4;
-                *reinterpret_cast<float4*>(v_s + key * DMAX + c) = v4;
-                odd |= !(fabsf(v4.x) < INFINITY && fabsf(v4.y) < INFINITY && fabsf(v4.z) < INFINITY && fabsf(v4.w) < INFINITY);
+            if (more) {
+                ask(base + KEYS, buffer ^ 1);
+                where_next = position_of(base + KEYS);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+            }
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {                   // (the pieces this thread brought)
+                const int e = tid + i * THREADS;
+                float v[EPP];
+                unpack<T>(*reinterpret_cast<const uint4*>(v_t + e / P * DMAX + e % P * EPP), v);
+#pragma unroll
+                for (int c = 0; c < EPP; ++c) odd |= !(fabsf(v[c]) < INFINITY);
             }
         } else {
+            if (more) where_next = position_of(base + KEYS);
             for (int e = tid; e < KEYS * DMAX; e += THREADS) {
                 const int key = e / DMAX, c = e % DMAX;
-                const long long at = key_at[key];
-                const bool there = at >= 0 && c < D;
-                k_s[key * PITCH + c] = there ? to_f32(((const T*)p.pages)[at + c]) : 0.0f;
-                const float v = there ? to_f32(((const T*)p.pages)[at + v_offset + c]) : 0.0f;
-                v_s[key * DMAX + c] = v;
-                odd |= !(fabsf(v) < INFINITY);
+                const long long at = c < D ? place_of(base + key) : -1;
+                const T k = at >= 0 ? ((const T*)p.pages)[at + c] : from_f32<T>(0.0f), v = at >= 0 ? ((const T*)p.pages)[at + v_offset + c] : from_f32<T>(0.0f);
+                k_s[(buffer * KEYS + key) * PITCH + c] = k;
+                v_s[(buffer * KEYS + key) * DMAX + c] = v;
+                odd |= !(fabsf(to_f32(v)) < INFINITY);
             }
         }
         odd = __syncthreads_or(odd);
         // scores: a lane a key, the warp's four rows
         float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const float* const k = k_s + lane * PITCH;
-#pragma unroll 8
-        for (int c = 0; c < DMAX; c += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(k + c);
+#pragma unroll 4
+        for (int c = 0; c < DMAX; c += EPP) {
+            float k[EPP];
+            unpack<T>(*reinterpret_cast<const uint4*>(k_t + lane * PITCH + c), k);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 q4 = *reinterpret_cast<const float4*>(q_s + (warp * 4 + i) * DMAX + c);
-                s[i] = fmaf(q4.x, k4.x, fmaf(q4.y, k4.y, fmaf(q4.z, k4.z, fmaf(q4.w, k4.w, s[i]))));
-            }
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < EPP; j += 4) {
+                    const float4 q4 = *reinterpret_cast<const float4*>(q_s + (warp * 4 + i) * DMAX + c + j);
+                    s[i] = fmaf(q4.x, k[j], fmaf(q4.y, k[j + 1], fmaf(q4.z, k[j + 2], fmaf(q4.w, k[j + 3], s[i]))));
+                }
         }
-        const int key = base + lane, where = key_pos_s[lane];
+        const int key = base + lane;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = warp * 4 + i;
@@ -227,6 +257,7 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
             p_s[r][lane] = e;
             if (lane == 0) alpha_s[r] = alpha;
         }
+        where = where_next;
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < RPT; ++r)
@@ -239,26 +270,26 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
                     const float e = p_s[my_row + r][j];
 #pragma unroll
                     for (int c = 0; c < COLS; ++c)
-                        if (e != 0.0f) acc[r][c] = fmaf(e, v_s[j * DMAX + my_col + c * 128], acc[r][c]);
+                        if (e != 0.0f) acc[r][c] = fmaf(e, to_f32(v_t[j * DMAX + my_col + c * 128]), acc[r][c]);
                 }
-            continue;
-        }
+        } else {
 #pragma unroll 2
-        for (int j = 0; j < KEYS; j += 4) {
-            float v[4][COLS];
+            for (int j = 0; j < KEYS; j += 4) {
+                float v[4][COLS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int c = 0; c < COLS; ++c) v[i][c] = v_s[(j + i) * DMAX + my_col + c * 128];
+                    for (int c = 0; c < COLS; ++c) v[i][c] = to_f32(v_t[(j + i) * DMAX + my_col + c * 128]);
 #pragma unroll
-            for (int r = 0; r < RPT; ++r) {
-                const float4 e = *reinterpret_cast<const float4*>(&p_s[my_row + r][j]);
+                for (int r = 0; r < RPT; ++r) {
+                    const float4 e = *reinterpret_cast<const float4*>(&p_s[my_row + r][j]);
 #pragma unroll
-                for (int c = 0; c < COLS; ++c) acc[r][c] = fmaf(e.w, v[3][c], fmaf(e.z, v[2][c], fmaf(e.y, v[1][c], fmaf(e.x, v[0][c], acc[r][c]))));
+                    for (int c = 0; c < COLS; ++c) acc[r][c] = fmaf(e.w, v[3][c], fmaf(e.z, v[2][c], fmaf(e.y, v[1][c], fmaf(e.x, v[0][c], acc[r][c]))));
+                }
             }
         }
+        __syncthreads();                                       // this tile's rows and weights were read
     }
-    __syncthreads();
     if (lane == 0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { sum_s[warp * 4 + i] = l[i]; max_s[warp * 4 + i] = m[i]; }
@@ -270,7 +301,7 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
         const int at = my_row + r;
         if (at >= rows) continue;
         const size_t row = (size_t)(start + (row0 + at) / G) * p.heads + kvh * G + (row0 + at) % G;
-        const float inv = sum_s[at] > 0.0f ? 1.0f / sum_s[at] : 0.0f;
+        const float inv = sum_s[at] > 0.0f ? 1.0f / sum_s[at] : sum_s[at] == sum_s[at] ? 0.0f : NAN;
 #pragma unroll
         for (int c = 0; c < COLS; ++c) {
             const int col = my_col + c * 128;
@@ -293,23 +324,26 @@ __global__ void __launch_bounds__(THREADS) draft_join_kernel(DraftParams p) {
     const size_t row = (size_t)start * p.heads + at, all_rows = (size_t)p.tokens * p.heads;
     const int length = p.lengths[seq], keys = length + n - first_key(length, p.window) / KEYS * KEYS;
     const int shares = min(p.shares, (keys + p.share - 1) / p.share);
-    float top = -INFINITY;
-    for (int s = lane; s < shares; s += 32) top = fmaxf(top, p.part_norm[s * all_rows + row].x);
+    const float2 mine = lane < shares ? p.part_norm[lane * all_rows + row] : make_float2(-INFINITY, 0.0f);       // of the first 32 shares
+    float top = mine.x;
+    for (int s = lane + 32; s < shares; s += 32) top = fmaxf(top, p.part_norm[s * all_rows + row].x);
     top = warp_max(top);
     float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0}, sum = 0.0f;
-    if (top > -INFINITY) {
-        for (int s = 0; s < shares; ++s) {
-            const float2 norm = p.part_norm[s * all_rows + row];
-            if (norm.x == -INFINITY) continue;
-            const float w = expf(norm.x - top);
-            sum += norm.y * w;
-            const float* const o = p.part_out + (s * all_rows + row) * p.dim;
+    for (int s0 = 0; s0 < shares; s0 += 32) {
+        const float2 norm = s0 == 0 ? mine : s0 + lane < shares ? p.part_norm[(s0 + lane) * all_rows + row] : make_float2(-INFINITY, 0.0f);
+        const float weight = norm.x == -INFINITY ? 0.0f : expf(norm.x - top), part = norm.x == -INFINITY ? (norm.y == norm.y ? 0.0f : NAN) : norm.y * weight;
+        const int here = min(32, shares - s0);
+#pragma unroll 4
+        for (int s = 0; s < here; ++s) {
+            const float w = __shfl_sync(0xffffffffu, weight, s);
+            sum += __shfl_sync(0xffffffffu, part, s);
+            const float* const o = p.part_out + ((size_t)(s0 + s) * all_rows + row) * p.dim;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                if (lane + 32 * i < p.dim) acc[i] = fmaf(w, o[lane + 32 * i], acc[i]);
+                if (w != 0.0f && lane + 32 * i < p.dim) acc[i] = fmaf(w, o[lane + 32 * i], acc[i]);
         }
     }
-    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : NAN;
     T* const out = (T*)p.out + row * p.dim;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -318,7 +352,7 @@ __global__ void __launch_bounds__(THREADS) draft_join_kernel(DraftParams p) {
 
 template <typename T, int DMAX, bool PIECES>
 int launch_attention(const DraftParams& p, int sequences, cudaStream_t stream) {
-    constexpr int bytes = (ROWS * DMAX + KEYS * (DMAX + 4) + KEYS * DMAX) * 4;
+    constexpr int bytes = attention_smem<T, DMAX>();
     static bool configured[MAX_DEVICES] = {};
     const int d = device_index();
     if (bytes > 40 * 1024 && !configured[d]) {
@@ -339,7 +373,7 @@ int launch_attention(const DraftParams& p, int sequences, cudaStream_t stream) {
 
 template <typename T>
 int run_attention(const DraftParams& p, int sequences, int max_nodes, cudaStream_t stream) {
-    const bool pieces = p.dim % 4 == 0 && ((uintptr_t)p.pages & 15) == 0;
+    const bool pieces = p.dim * sizeof(T) % 16 == 0 && ((uintptr_t)p.pages & 15) == 0;
     const int status = pieces ? launch_attention<T, true>(p, sequences, stream) : launch_attention<T, false>(p, sequences, stream);
     if (status != MLB_OK || p.shares == 1) return status;
     const int rows = THREADS / 32;

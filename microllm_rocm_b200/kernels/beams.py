@@ -8,7 +8,7 @@ import torch
 
 from . import build, ops
 from .build import KernelError
-from .cache_moves import need_current, need_on
+from .cache_moves import INT, need_current, need_on
 
 MAX_BEAMS = 32              # csrc/beams.cu
 MAX_WANTED = 64
@@ -23,7 +23,7 @@ ops.register_signatures("beams.cu", {
 def _scratch_bytes(rows: int, vocab: int, wanted: int) -> int:
     slots = rows * -(-vocab // SLICE)
     up = lambda n: -(-n // 16) * 16
-    return up(slots * 8) + 2 * up(slots * 4) + 2 * up(slots * wanted * 4)
+    return 2 * up(slots * 8) + up(slots * 4) + 2 * up(slots * wanted * 4)
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, out_scores: torch.Tensor, out_parents: torch.Tensor, out_tokens: torch.Tensor,
@@ -41,17 +41,15 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, out_scores: torch.Te
     if logits.dim() != 2 or logits.stride(1) != 1 or (logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]):
         raise KernelError("beam_select: logits are rows of neighbouring elements that do not overlap")
     tag = ops.dtype_tag(logits)
-    need_on(device, scores, "scores", torch.float32, 2)
-    need_on(device, out_scores, "out_scores", torch.float32, 2)
-    need_on(device, out_parents, "out_parents", torch.int32, 2)
-    need_on(device, out_tokens, "out_tokens", torch.int32, 2)
+    need_on(device, (scores, "scores", torch.float32, 2), (out_scores, "out_scores", torch.float32, 2), (out_parents, "out_parents", INT, 2),
+            (out_tokens, "out_tokens", INT, 2))
     (requests, beams), (rows, vocab), wanted = scores.shape, logits.shape, out_scores.shape[1]
     if rows != requests * beams or out_scores.shape[0] != requests or out_parents.shape != out_scores.shape or out_tokens.shape != out_scores.shape:
         raise KernelError("beam_select: one row of logits per beam, one row of outputs per request")
     if not 0 < beams <= MAX_BEAMS or not 0 < wanted <= MAX_WANTED or vocab == 0:
         raise KernelError(f"beam_select: {beams} beams and {wanted} continuations of {vocab} tokens (1 to {MAX_BEAMS} and 1 to {MAX_WANTED})")
     if ended is not None:
-        need_on(device, ended, "ended", torch.int32, 2)
+        need_on(device, (ended, "ended", INT, 2))
         if ended.shape != scores.shape:
             raise KernelError("beam_select: one `ended` per beam")
         if not 0 <= end_token < vocab:

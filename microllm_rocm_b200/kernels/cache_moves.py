@@ -17,6 +17,7 @@ from .build import KernelError
 
 MAX_STORAGES = 128          # csrc/cache_moves.cu: MAX_STORAGES
 MAX_BEAMS = 32              # csrc/cache_moves.cu: MAX_BEAMS
+INT = torch.int32
 
 _PAGES = [c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_int]          # bases, count, pages, page size, planes, row, planes2, row2
 
@@ -94,10 +95,11 @@ class PageMoves(_Storages):
         self._gather(tensors, layouts)
 
 
-def need_on(device_index: int, t: torch.Tensor, name: str, dtype, dims: int) -> None:
-    """`t` is a contiguous tensor of that type on the device of the call's other tensors."""
-    if t.get_device() != device_index or t.dtype != dtype or t.dim() != dims or not t.is_contiguous():
-        raise KernelError(f"{name} must be a contiguous {dtype} tensor of {dims} dimensions on the call's device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+def need_on(device_index: int, *tensors) -> None:
+    """Each of the (tensor, name, type, dimensions) is a contiguous tensor of that type on the device of the call's other tensors."""
+    for t, name, dtype, dims in tensors:
+        if t.dtype is not dtype or t.get_device() != device_index or t.dim() != dims or not t.is_contiguous():
+            raise KernelError(f"{name} must be a contiguous {dtype} tensor of {dims} dimensions on the call's device, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def need_current(device_index: int, what: str) -> None:
@@ -110,7 +112,7 @@ def need_current(device_index: int, what: str) -> None:
 
 
 def _need_beams(device: int, parents: torch.Tensor, what: str) -> Tuple[int, int]:
-    need_on(device, parents, "parents", torch.int32, 2)
+    need_on(device, (parents, "parents", INT, 2))
     requests, beams = parents.shape
     if not 0 < beams <= MAX_BEAMS:
         raise KernelError(f"{what}: {beams} beams (1 to {MAX_BEAMS})")
@@ -127,11 +129,11 @@ def reorder_slots(moves: SlotMoves, slots: torch.Tensor, parents: torch.Tensor, 
         return
     device = moves.device_index
     requests, beams = _need_beams(device, parents, "reorder_slots")
-    need_on(device, slots, "slots", torch.int32, 2)
+    need_on(device, (slots, "slots", INT, 2))
     if slots.shape != parents.shape:
         raise KernelError("reorder_slots: one slot and one parent per beam")
     if error_flag is not None:
-        need_on(device, error_flag, "error_flag", torch.int32, 1)
+        need_on(device, (error_flag, "error_flag", INT, 1))
     need_current(device, "reorder_slots")
     L = ops.lib("cache_moves.cu")
     for address, count, layout, _ in moves.groups:
@@ -151,15 +153,13 @@ def reorder_pages(moves: PageMoves, block_table: torch.Tensor, parents: torch.Te
         return
     device = moves.device_index
     requests, beams = _need_beams(device, parents, "reorder_pages")
-    need_on(device, block_table, "block_table", torch.int32, 2)
-    need_on(device, first, "first", torch.int32, 1)
-    need_on(device, last, "last", torch.int32, 1)
+    need_on(device, (block_table, "block_table", INT, 2), (first, "first", INT, 1), (last, "last", INT, 1))
     if block_table.shape[0] != requests * beams or first.shape[0] != requests or last.shape[0] != requests:
         raise KernelError("reorder_pages: one row of the block table per beam, one first and last token per request")
     if max_tokens < 0 or max_tokens > block_table.shape[1] * moves.page_size:
         raise KernelError(f"reorder_pages: {max_tokens} tokens do not fit {block_table.shape[1]} blocks of {moves.page_size}")
     if error_flag is not None:
-        need_on(device, error_flag, "error_flag", torch.int32, 1)
+        need_on(device, (error_flag, "error_flag", INT, 1))
     if requests == 0 or max_tokens == 0:
         return
     need_current(device, "reorder_pages")

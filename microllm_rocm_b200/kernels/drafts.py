@@ -15,7 +15,7 @@ import torch
 
 from . import build, ops
 from .build import KernelError
-from .cache_moves import PageMoves, need_current, need_on
+from .cache_moves import INT, PageMoves, need_current, need_on
 from .device import sm_count
 
 MAX_NODES = 256             # csrc/drafts.cu: nodes of a sequence
@@ -35,6 +35,17 @@ ops.register_signatures("drafts_tc.cu", {
 })
 
 
+_TC_DEFINES = {d: {"HEAD_DIM": d} for d in TC_HEAD_DIMS}
+_sms = {}
+
+
+def _sm_count(device_index: int) -> int:
+    got = _sms.get(device_index)
+    if got is None:
+        got = _sms[device_index] = sm_count(torch.device("cuda", device_index))
+    return got
+
+
 def tc_sources(head_dim: int):
     return [("drafts_tc.cu", {"HEAD_DIM": head_dim})] if head_dim in TC_HEAD_DIMS else []
 
@@ -45,8 +56,7 @@ def tc_supported(head_dim: int, page_size: int, group: int, scale: float) -> boo
 
 
 def _need_trees(device: int, starts: torch.Tensor, lengths: torch.Tensor) -> int:
-    need_on(device, starts, "starts", torch.int32, 1)
-    need_on(device, lengths, "lengths", torch.int32, 1)
+    need_on(device, (starts, "starts", INT, 1), (lengths, "lengths", INT, 1))
     if starts.shape[0] != lengths.shape[0] + 1:
         raise KernelError("drafts: `starts` has one entry per sequence and one more")
     return lengths.shape[0]
@@ -59,19 +69,17 @@ def draft_masks(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tens
     most 8.  A parent that is not an earlier node counts as none and raises the error flag; a sequence of more nodes than the masks hold
     raises it too and is left out."""
     device = parents.get_device()
-    need_on(device, parents, "parents", torch.int32, 1)
+    need_on(device, (parents, "parents", INT, 1), (masks, "masks", INT, 2), (positions, "positions", INT, 1))
     sequences = _need_trees(device, starts, lengths)
-    need_on(device, masks, "masks", torch.int32, 2)
-    need_on(device, positions, "positions", torch.int32, 1)
     T = parents.shape[0]
     if masks.shape[0] != T or positions.shape[0] != T or not 0 < masks.shape[1] <= MAX_NODES // 32:
         raise KernelError(f"draft_masks: one row of 1 to {MAX_NODES // 32} words and one position per node")
     if places is not None:
-        need_on(device, places, "places", torch.int32, 1)
+        need_on(device, (places, "places", INT, 1))
         if places.shape[0] != T:
             raise KernelError("draft_masks: one place per node")
     if error_flag is not None:
-        need_on(device, error_flag, "error_flag", torch.int32, 1)
+        need_on(device, (error_flag, "error_flag", INT, 1))
     need_current(device, "draft_masks")
     L = ops.lib("drafts.cu")
     build.check(L, L.mlb_draft_masks(parents.data_ptr(), starts.data_ptr(), lengths.data_ptr(), sequences, masks.shape[1], masks.data_ptr(), positions.data_ptr(),
@@ -101,21 +109,17 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     `max_nodes`: the most nodes of a sequence, which the launch is sized for (a sequence of more raises the error flag).  `max_length`: the most keys
     of a sequence, its nodes among them (how the work is cut; a longer sequence costs time only)."""
     device = q.get_device()
-    tag = ops.dtype_tag(q)
-    need_on(device, q, "q", q.dtype, 2)
-    need_on(device, pages, "pages", q.dtype, 5)
-    need_on(device, out, "out", q.dtype, 2)
+    tag, dtype = ops.dtype_tag(q), q.dtype
+    need_on(device, (q, "q", dtype, 2), (pages, "pages", dtype, 5), (out, "out", dtype, 2), (positions, "positions", INT, 1), (masks, "masks", INT, 2),
+            (block_table, "block_table", INT, 2))
     sequences = _need_trees(device, starts, lengths)
-    need_on(device, positions, "positions", torch.int32, 1)
-    need_on(device, masks, "masks", torch.int32, 2)
-    need_on(device, block_table, "block_table", torch.int32, 2)
-    T = q.shape[0]
+    T, width = q.shape
     num_pages, two, nkv, page_size, d = pages.shape
     if two != 2 or nkv != num_kv_heads or d != head_dim:
         raise KernelError(f"draft_attention: pages {tuple(pages.shape)} do not match the head geometry")
     if num_kv_heads <= 0 or num_heads % num_kv_heads or not 0 < head_dim <= 256:
         raise KernelError(f"draft_attention: heads {num_heads}/{num_kv_heads} of {head_dim}")
-    if q.shape[1] != num_heads * head_dim or out.shape != q.shape or positions.shape[0] != T or masks.shape[0] != T or block_table.shape[0] != sequences:
+    if width != num_heads * head_dim or out.shape != q.shape or positions.shape[0] != T or masks.shape[0] != T or block_table.shape[0] != sequences:
         raise KernelError("draft_attention: shapes do not agree")
     words = masks.shape[1]
     if not 0 < words <= MAX_NODES // 32 or not 0 < max_nodes <= words * 32 or max_length < max_nodes:
@@ -123,27 +127,28 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     if window is not None and window <= 0:
         raise KernelError("draft_attention: a window has at least one key")
     if error_flag is not None:
-        need_on(device, error_flag, "error_flag", torch.int32, 1)
+        need_on(device, (error_flag, "error_flag", INT, 1))
     if T == 0 or sequences == 0:
         return
     need_current(device, "draft_attention")
     group = num_heads // num_kv_heads
-    if q.dtype == torch.bfloat16 and tc_supported(head_dim, page_size, group, scale) and not (q.data_ptr() | pages.data_ptr() | out.data_ptr()) & 15:
+    q_at, pages_at, out_at = q.data_ptr(), pages.data_ptr(), out.data_ptr()
+    if dtype is torch.bfloat16 and tc_supported(head_dim, page_size, group, scale) and not (q_at | pages_at | out_at) & 15:
         keys = min(max_length, window + max_nodes + TC_KEYS) if window else max_length
-        ctas = _ctas(sequences * num_kv_heads, -(-max_nodes // (TC_ROWS // group)), -(-keys // TC_KEYS), sm_count(q.device))
+        ctas = _ctas(sequences * num_kv_heads, -(-max_nodes // (TC_ROWS // group)), -(-keys // TC_KEYS), _sm_count(device))
         scratch = ops.scratch(ctas * 4 * TC_ROWS * (head_dim + 2) * 4 + 8 + 4 * sequences, q.device, "draft_attention") if ctas > 1 else None
-        L = ops.lib("drafts_tc.cu", {"HEAD_DIM": head_dim})
-        build.check(L, L.mlb_draft_attention_tc(q.data_ptr(), pages.data_ptr(), out.data_ptr(), starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
+        L = ops.lib("drafts_tc.cu", _TC_DEFINES[head_dim])
+        build.check(L, L.mlb_draft_attention_tc(q_at, pages_at, out_at, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
                                                 masks.data_ptr(), words, block_table.data_ptr(), block_table.shape[1], num_pages, page_size, T, sequences,
                                                 int(max_nodes), num_heads, num_kv_heads, float(scale), int(window or 0), TC_STRETCH, ctas, ops._ptr(scratch),
                                                 ops._ptr(error_flag), ops._stream()))
         return
     keys = min(max_length, window + max_nodes + KEYS) if window else max_length
     row_tiles = -(-max_nodes * group // ROWS)
-    share, shares = _shares(sequences * num_kv_heads * row_tiles, keys, sm_count(q.device))
+    share, shares = _shares(sequences * num_kv_heads * row_tiles, keys, _sm_count(device))
     scratch = ops.scratch(shares * T * num_heads * (head_dim + 2) * 4, q.device, "draft_attention") if shares > 1 else None
     L = ops.lib("drafts.cu")
-    build.check(L, L.mlb_draft_attention(q.data_ptr(), pages.data_ptr(), out.data_ptr(), tag, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
+    build.check(L, L.mlb_draft_attention(q_at, pages_at, out_at, tag, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
                                          masks.data_ptr(), words, block_table.data_ptr(), block_table.shape[1], num_pages, page_size, T, sequences, int(max_nodes),
                                          num_heads, num_kv_heads, head_dim, float(scale), int(window or 0), share, shares, ops._ptr(scratch),
                                          ops._ptr(error_flag), ops._stream()))
@@ -158,25 +163,22 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
     move from place lengths[a] + path[a, i] to lengths[a] + i, so that the cache holds the branch as if it had been decoded token by
     token.  All int32.  A sequence without nodes gets a count of 0; one of more than `width` or 256 nodes raises the error flag."""
     device = tokens.get_device()
-    for t, name in ((tokens, "tokens"), (parents, "parents"), (choices, "choices")):
-        need_on(device, t, name, torch.int32, 1)
+    need_on(device, (tokens, "tokens", INT, 1), (parents, "parents", INT, 1), (choices, "choices", INT, 1), (path, "path", INT, 2), (counts, "counts", INT, 1),
+            (following, "following", INT, 1))
     sequences = _need_trees(device, starts, lengths)
-    need_on(device, path, "path", torch.int32, 2)
-    need_on(device, counts, "counts", torch.int32, 1)
-    need_on(device, following, "following", torch.int32, 1)
     if parents.shape != tokens.shape or choices.shape != tokens.shape:
         raise KernelError("accept_drafts: one token, parent and choice per node")
     if path.shape[0] != sequences or path.shape[1] == 0 or counts.shape[0] != sequences or following.shape[0] != sequences:
         raise KernelError("accept_drafts: one path, count and following token per sequence")
     if error_flag is not None:
-        need_on(device, error_flag, "error_flag", torch.int32, 1)
+        need_on(device, (error_flag, "error_flag", INT, 1))
     groups = []
     if moves is not None:
         if not isinstance(moves, PageMoves):
             raise KernelError("accept_drafts moves the storages of a PageMoves")
         if block_table is None:
             raise KernelError("accept_drafts: moving rows takes a block table")
-        need_on(device, block_table, "block_table", torch.int32, 2)
+        need_on(device, (block_table, "block_table", INT, 2))
         if block_table.shape[0] != sequences or (moves.groups and moves.device_index != device):
             raise KernelError("accept_drafts: one row of the block table per sequence, and pools on the same device")
         groups = moves.groups

@@ -725,9 +725,9 @@ def second_stream():
 def scratch(nbytes: int, device: torch.device, what: str) -> torch.Tensor:
     """Memory for one call's own use between its launches: the tensor framework's, which takes it back in the order of the current stream.  A
     launch on the second stream is not in that order, so there it is the step's (`on_side_stream(scratch)`)."""
-    side, step_scratch = second_stream()
-    if side is None:
+    if getattr(_launch_on, "side", None) is None:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    step_scratch = getattr(_launch_on, "scratch", None)
     if step_scratch is None:
         raise KernelError(f"{what}: on the second stream it needs the step's scratch memory (on_side_stream(scratch))")
     return step_scratch(nbytes)

@@ -79,7 +79,8 @@ def select(logits, scores, wanted, ended=None, end_token=-1):
         row = logits[b].double()
         if math.isnan(score) or score == math.inf or bool((~(row < math.inf)).any()):
             return [math.nan] * wanted, [-1] * wanted, [-1] * wanted
-        row = row - torch.logsumexp(row, 0)
+        row = row - row.max().clamp(min=torch.finfo(torch.float32).min)      # first, so that a row of the type's lowest values keeps its normaliser
+        row = row - row.exp().sum().log()
         found += [(-(score + x), b, t) for t, x in enumerate(row.tolist()) if x > -math.inf]
     found = sorted(found)[:wanted]
     found += [(math.inf, -1, -1)] * (wanted - len(found))
