@@ -59,9 +59,12 @@ __global__ void __launch_bounds__(MAX_NODES) draft_masks_kernel(const int* __res
 }
 
 // ------------------------------------------------------------------------------ attention
-constexpr int THREADS = 128;
-constexpr int ROWS = 16;                       // (node, head) rows of one kv head a CTA works on; a warp has four
+constexpr int THREADS = 128;                   // of a group: four warps that share a tile of keys
+constexpr int ROWS = 16;                       // (node, head) rows of one kv head a CTA works on; a warp of a group has four
 constexpr int KEYS = 32;                       // keys a tile: a lane each
+// What bounds these sizes is the way of one warp through a tile, not the arithmetic or the memory, so a CTA has several groups, each with a tile of its own, and they
+// join in shared memory.  (As many as fit it: two for fp32 heads beyond 128.)
+template <typename T, int DMAX> constexpr int groups() { return DMAX * (int)sizeof(T) > 512 ? 2 : 4; }
 
 struct DraftParams {
     const void* q;           // [T, ldq]
@@ -97,35 +100,44 @@ template <typename T> __device__ __forceinline__ void unpack(const uint4& x, flo
     }
 }
 
-template <typename T, int DMAX> constexpr int attention_smem() {
-    return ROWS * DMAX * 4 + 2 * KEYS * (2 * DMAX + 16 / (int)sizeof(T)) * (int)sizeof(T);
+template <typename T, int DMAX> constexpr int tile_bytes() { return KEYS * (2 * DMAX + 16 / (int)sizeof(T)) * (int)sizeof(T); }
+template <typename T, int DMAX> constexpr int attention_smem() { return ROWS * DMAX * 4 + groups<T, DMAX>() * tile_bytes<T, DMAX>(); }
+
+__device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(THREADS) : "memory"); }
+__device__ __forceinline__ bool group_or(int group, bool mine) {
+    int any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any) : "r"(mine ? 1 : 0), "r"(group + 1), "n"(THREADS) : "memory");
+    return any != 0;
 }
 
 template <typename T, int DMAX, bool PIECES>
-__global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p) {
+__global__ void __launch_bounds__(groups<T, DMAX>() * THREADS, 1) draft_attention_kernel(DraftParams p) {
     pdl_prologue();
+    constexpr int GROUPS = groups<T, DMAX>();
     constexpr int COLS = DMAX > 128 ? 2 : 1;
     constexpr int RPT = DMAX >= 128 ? ROWS : DMAX / 8;         // 32: 4, 64: 8
     constexpr int EPP = 16 / sizeof(T);                        // elements a piece
     constexpr int PITCH = DMAX + EPP;                          // of a key row: neighbouring lanes' pieces in different banks
-    constexpr int P = DMAX / EPP, MINE = KEYS * P / THREADS > 0 ? KEYS * P / THREADS : 1;      // pieces of a row, and a thread's of a tile
+    constexpr int P = DMAX / EPP, MINE = KEYS * P / THREADS;   // pieces of a row, and a thread's of a tile
     static_assert(KEYS * P % THREADS == 0, "whole rounds of pieces");
+    static_assert(ROWS * DMAX * 4 <= tile_bytes<T, DMAX>(), "a group's result fits where its tile was");
     extern __shared__ __align__(16) unsigned char smem[];
     float* const q_s = reinterpret_cast<float*>(smem);         // [ROWS][DMAX]
-    T* const k_s = reinterpret_cast<T*>(q_s + ROWS * DMAX);    // [2][KEYS][PITCH]
-    T* const v_s = k_s + 2 * KEYS * PITCH;                     // [2][KEYS][DMAX]
-    __shared__ __align__(16) float p_s[ROWS][KEYS];
-    __shared__ float alpha_s[ROWS], sum_s[ROWS], max_s[ROWS];
+    __shared__ __align__(16) float p_s[GROUPS][ROWS][KEYS];
+    __shared__ float alpha_s[GROUPS][ROWS], sum_s[GROUPS][ROWS], max_s[GROUPS][ROWS];
     __shared__ unsigned mask_s[ROWS][MAX_WORDS];
     __shared__ int pos_s[ROWS];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int lane = threadIdx.x & 31, group = threadIdx.x / THREADS, tid = threadIdx.x % THREADS, warp = tid >> 5;
+    T* const k_s = reinterpret_cast<T*>(smem + ROWS * DMAX * 4 + group * tile_bytes<T, DMAX>());      // [KEYS][PITCH]
+    T* const v_s = k_s + KEYS * PITCH;                         // [KEYS][DMAX]
     const int share = blockIdx.x, seq = blockIdx.z;
     const int kvh = blockIdx.y / p.row_tiles, row0 = (blockIdx.y % p.row_tiles) * ROWS;
     const int start = p.starts[seq], n = p.starts[seq + 1] - start, length = p.lengths[seq];
     const int G = p.group, D = p.dim;
     const int rows = min(ROWS, n * G - row0);
     if (rows <= 0) return;
-    if (n > p.max_nodes && tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);      // the grid has no rows for the last of them
+    if (n > p.max_nodes && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 3);      // the grid has no rows for the last of them
     // The shares begin at the first key that a row may see (positions are at least `length`); the last one takes what is left, so that a
     // sequence longer than the caller said costs time and nothing else.
     const int lo = first_key(length, p.window), total = length + n;
@@ -135,7 +147,7 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
 
     const size_t plane = (size_t)p.page_size * D, page_stride = 2 * plane * p.kv_heads, v_offset = plane * p.kv_heads;
     const int* const table = p.table + (size_t)seq * p.max_blocks;
-    // where a key's row begins in the pool; -1: no row may see it, or it has no page
+    // where the row of the lane's key begins in the pool; -1: no row may see it, or it has no page
     auto place_of = [&](int key) -> long long {
         if (key < lo || key >= key_end) return -1;
         const int block = key / p.page_size;
@@ -146,41 +158,31 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
         }
         return (long long)((size_t)page * page_stride + (size_t)kvh * plane + (size_t)(key % p.page_size) * D);
     };
-    auto ask = [&](int base, int buffer) {                     // the pieces of a tile's keys and values
-        long long at[MINE];
-#pragma unroll
-        for (int i = 0; i < MINE; ++i) at[i] = place_of(base + (tid + i * THREADS) / P);
+    auto ask = [&](long long place) {                          // the pieces of a tile's keys and values
 #pragma unroll
         for (int i = 0; i < MINE; ++i) {
             const int e = tid + i * THREADS, key = e / P, c = e % P * EPP;
-            const bool there = at[i] >= 0 && c < D;
-            const T* const from = (const T*)p.pages + (there ? at[i] + c : 0);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(k_s + (buffer * KEYS + key) * PITCH + c)), "l"(from),
+            const long long at = __shfl_sync(0xffffffffu, place, key);
+            const bool there = at >= 0 && c < D;
+            const T* const from = (const T*)p.pages + (there ? at + c : 0);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(k_s + key * PITCH + c)), "l"(from),
                          "r"(there ? 16 : 0) : "memory");
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(v_s + (buffer * KEYS + key) * DMAX + c)), "l"(from + (there ? v_offset : 0)),
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(v_s + key * DMAX + c)), "l"(from + (there ? v_offset : 0)),
                          "r"(there ? 16 : 0) : "memory");
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // the position of the lane's key; -1: not there
-    auto position_of = [&](int base) { return place_of(base + lane) < 0 ? -1 : base + lane < length ? base + lane : p.positions[start + base + lane - length]; };
-
-    if (PIECES) ask(key_begin, 0);
-    int where = position_of(key_begin);
-    for (int e = tid; e < ROWS * DMAX; e += THREADS) {
-        const int r = e / DMAX, c = e % DMAX;
-        float v = 0.0f;
-        if (r < rows && c < D) {
-            const int row = row0 + r;
-            v = to_f32(((const T*)p.q)[(size_t)(start + row / G) * p.heads * D + (size_t)(kvh * G + row % G) * D + c]);
-        }
-        q_s[e] = v;
+    const int first = key_begin + group * KEYS;
+    long long place = place_of(first + lane);
+    if (PIECES && first < key_end) ask(place);
+    for (int r = threadIdx.x >> 5; r < ROWS; r += GROUPS * THREADS / 32) {
+        const int node = start + (row0 + min(r, rows - 1)) / G, head = kvh * G + (row0 + min(r, rows - 1)) % G;
+        const T* const q = (const T*)p.q + ((size_t)node * p.heads + head) * D;
+#pragma unroll
+        for (int c = lane; c < DMAX; c += 32) q_s[r * DMAX + c] = r < rows && c < D ? to_f32(q[c]) : 0.0f;
+        if (lane < p.words) mask_s[r][lane] = r < rows ? (unsigned)p.masks[(size_t)node * p.words + lane] : 0u;
+        if (lane == 0) pos_s[r] = p.positions[node];
     }
-    for (int e = tid; e < ROWS * p.words; e += THREADS) {
-        const int r = e / p.words, w = e % p.words;
-        mask_s[r][w] = r < rows ? (unsigned)p.masks[(size_t)(start + (row0 + r) / G) * p.words + w] : 0u;
-    }
-    if (tid < ROWS) pos_s[tid] = tid < rows ? p.positions[start + (row0 + tid) / G] : 0;
+    __syncthreads();
 
     float acc[RPT][COLS];
 #pragma unroll
@@ -193,47 +195,40 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
 #pragma unroll
     for (int i = 0; i < 4; ++i) { m[i] = -INFINITY; l[i] = 0.0f; }
 
-    int buffer = 0;
-    for (int base = key_begin; base < key_end; base += KEYS, buffer ^= 1) {
-        const bool more = base + KEYS < key_end;
-        const T* const k_t = k_s + buffer * KEYS * PITCH;
-        const T* const v_t = v_s + buffer * KEYS * DMAX;
+    for (int base = first; base < key_end; base += GROUPS * KEYS) {
+        const int key = base + lane;
+        const int where = place < 0 ? -1 : key < length ? key : p.positions[start + key - length];      // the position of the lane's key; -1: not there
         bool odd = false;                                      // a value that is not finite: it may not meet the zero weight of a row that does not see it
-        int where_next = -1;
         if (PIECES) {
-            if (more) {
-                ask(base + KEYS, buffer ^ 1);
-                where_next = position_of(base + KEYS);
-                asm volatile("cp.async.wait_group 1;" ::: "memory");
-            } else {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {                   // (the pieces this thread brought)
                 const int e = tid + i * THREADS;
                 float v[EPP];
-                unpack<T>(*reinterpret_cast<const uint4*>(v_t + e / P * DMAX + e % P * EPP), v);
+                unpack<T>(*reinterpret_cast<const uint4*>(v_s + e / P * DMAX + e % P * EPP), v);
 #pragma unroll
                 for (int c = 0; c < EPP; ++c) odd |= !(fabsf(v[c]) < INFINITY);
             }
         } else {
-            if (more) where_next = position_of(base + KEYS);
-            for (int e = tid; e < KEYS * DMAX; e += THREADS) {
-                const int key = e / DMAX, c = e % DMAX;
-                const long long at = c < D ? place_of(base + key) : -1;
-                const T k = at >= 0 ? ((const T*)p.pages)[at + c] : from_f32<T>(0.0f), v = at >= 0 ? ((const T*)p.pages)[at + v_offset + c] : from_f32<T>(0.0f);
-                k_s[(buffer * KEYS + key) * PITCH + c] = k;
-                v_s[(buffer * KEYS + key) * DMAX + c] = v;
-                odd |= !(fabsf(to_f32(v)) < INFINITY);
+            for (int j = warp; j < KEYS; j += THREADS / 32) {
+                const long long at = __shfl_sync(0xffffffffu, place, j);
+                for (int c = lane; c < DMAX; c += 32) {
+                    const bool there = at >= 0 && c < D;
+                    const T k = there ? ((const T*)p.pages)[at + c] : from_f32<T>(0.0f), v = there ? ((const T*)p.pages)[at + v_offset + c] : from_f32<T>(0.0f);
+                    k_s[j * PITCH + c] = k;
+                    v_s[j * DMAX + c] = v;
+                    odd |= !(fabsf(to_f32(v)) < INFINITY);
+                }
             }
         }
-        odd = __syncthreads_or(odd);
+        odd = group_or(group, odd);
+        place = place_of(key + GROUPS * KEYS);                 // of the next tile, on its way
         // scores: a lane a key, the warp's four rows
         float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
         for (int c = 0; c < DMAX; c += EPP) {
             float k[EPP];
-            unpack<T>(*reinterpret_cast<const uint4*>(k_t + lane * PITCH + c), k);
+            unpack<T>(*reinterpret_cast<const uint4*>(k_s + lane * PITCH + c), k);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -242,7 +237,6 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
                     s[i] = fmaf(q4.x, k[j], fmaf(q4.y, k[j + 1], fmaf(q4.z, k[j + 2], fmaf(q4.w, k[j + 3], s[i]))));
                 }
         }
-        const int key = base + lane;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = warp * 4 + i;
@@ -254,23 +248,22 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
             const float alpha = m[i] == -INFINITY ? 0.0f : expf(m[i] - m_new);
             l[i] = l[i] * alpha + warp_sum(e);
             m[i] = m_new;
-            p_s[r][lane] = e;
-            if (lane == 0) alpha_s[r] = alpha;
+            p_s[group][r][lane] = e;
+            if (lane == 0) alpha_s[group][r] = alpha;
         }
-        where = where_next;
-        __syncthreads();
+        group_sync(group);
 #pragma unroll
         for (int r = 0; r < RPT; ++r)
 #pragma unroll
-            for (int c = 0; c < COLS; ++c) acc[r][c] *= alpha_s[my_row + r];
+            for (int c = 0; c < COLS; ++c) acc[r][c] *= alpha_s[group][my_row + r];
         if (odd) {
             for (int j = 0; j < KEYS; ++j)
 #pragma unroll
                 for (int r = 0; r < RPT; ++r) {
-                    const float e = p_s[my_row + r][j];
+                    const float e = p_s[group][my_row + r][j];
 #pragma unroll
                     for (int c = 0; c < COLS; ++c)
-                        if (e != 0.0f) acc[r][c] = fmaf(e, to_f32(v_t[j * DMAX + my_col + c * 128]), acc[r][c]);
+                        if (e != 0.0f) acc[r][c] = fmaf(e, to_f32(v_s[j * DMAX + my_col + c * 128]), acc[r][c]);
                 }
         } else {
 #pragma unroll 2
@@ -279,37 +272,50 @@ __global__ void __launch_bounds__(THREADS) draft_attention_kernel(DraftParams p)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int c = 0; c < COLS; ++c) v[i][c] = to_f32(v_t[(j + i) * DMAX + my_col + c * 128]);
+                    for (int c = 0; c < COLS; ++c) v[i][c] = to_f32(v_s[(j + i) * DMAX + my_col + c * 128]);
 #pragma unroll
                 for (int r = 0; r < RPT; ++r) {
-                    const float4 e = *reinterpret_cast<const float4*>(&p_s[my_row + r][j]);
+                    const float4 e = *reinterpret_cast<const float4*>(&p_s[group][my_row + r][j]);
 #pragma unroll
                     for (int c = 0; c < COLS; ++c) acc[r][c] = fmaf(e.w, v[3][c], fmaf(e.z, v[2][c], fmaf(e.y, v[1][c], fmaf(e.x, v[0][c], acc[r][c]))));
                 }
             }
         }
-        __syncthreads();                                       // this tile's rows and weights were read
+        group_sync(group);                                     // this tile's rows and weights were read
+        if (PIECES && base + GROUPS * KEYS < key_end) ask(place);
     }
+    // the groups join
     if (lane == 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { sum_s[warp * 4 + i] = l[i]; max_s[warp * 4 + i] = m[i]; }
+        for (int i = 0; i < 4; ++i) { sum_s[group][warp * 4 + i] = l[i]; max_s[group][warp * 4 + i] = m[i]; }
     }
+    float* const mine_s = reinterpret_cast<float*>(k_s);       // [ROWS][DMAX]
+#pragma unroll
+    for (int r = 0; r < RPT; ++r)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) mine_s[(my_row + r) * DMAX + my_col + c * 128] = acc[r][c];
     __syncthreads();
     const size_t all_rows = (size_t)p.tokens * p.heads;
+    for (int e = threadIdx.x; e < rows * DMAX; e += GROUPS * THREADS) {
+        const int r = e / DMAX, col = e % DMAX;
+        if (col >= D) continue;
+        float top = -INFINITY, sum = 0.0f, o = 0.0f;
 #pragma unroll
-    for (int r = 0; r < RPT; ++r) {
-        const int at = my_row + r;
-        if (at >= rows) continue;
-        const size_t row = (size_t)(start + (row0 + at) / G) * p.heads + kvh * G + (row0 + at) % G;
-        const float inv = sum_s[at] > 0.0f ? 1.0f / sum_s[at] : sum_s[at] == sum_s[at] ? 0.0f : NAN;
+        for (int g = 0; g < GROUPS; ++g) top = fmaxf(top, max_s[g][r]);
 #pragma unroll
-        for (int c = 0; c < COLS; ++c) {
-            const int col = my_col + c * 128;
-            if (col >= D) continue;
-            if (p.shares == 1) ((T*)p.out)[row * D + col] = from_f32<T>(acc[r][c] * inv);
-            else p.part_out[((size_t)share * all_rows + row) * D + col] = acc[r][c];
+        for (int g = 0; g < GROUPS; ++g) {
+            const float w = max_s[g][r] == -INFINITY ? 0.0f : expf(max_s[g][r] - top);
+            sum += sum_s[g][r] == sum_s[g][r] ? sum_s[g][r] * w : NAN;
+            if (w != 0.0f) o = fmaf(w, reinterpret_cast<const float*>(smem + ROWS * DMAX * 4 + g * tile_bytes<T, DMAX>())[e], o);
         }
-        if (p.shares > 1 && my_col == 0) p.part_norm[(size_t)share * all_rows + row] = make_float2(max_s[at], sum_s[at]);
+        const size_t row = (size_t)(start + (row0 + r) / G) * p.heads + kvh * G + (row0 + r) % G;
+        if (p.shares == 1) {
+            const float inv = sum > 0.0f ? 1.0f / sum : sum == sum ? 0.0f : NAN;
+            ((T*)p.out)[row * D + col] = from_f32<T>(o * inv);
+        } else {
+            p.part_out[((size_t)share * all_rows + row) * D + col] = o;
+            if (col == 0) p.part_norm[(size_t)share * all_rows + row] = make_float2(top, sum);
+        }
     }
 }
 
@@ -355,12 +361,12 @@ int launch_attention(const DraftParams& p, int sequences, cudaStream_t stream) {
     constexpr int bytes = attention_smem<T, DMAX>();
     static bool configured[MAX_DEVICES] = {};
     const int d = device_index();
-    if (bytes > 40 * 1024 && !configured[d]) {
+    if (!configured[d]) {
         if (cudaFuncSetAttribute(draft_attention_kernel<T, DMAX, PIECES>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
             return check_launch("draft_attention: shared memory");
         configured[d] = true;
     }
-    launch_kernel(draft_attention_kernel<T, DMAX, PIECES>, dim3(p.shares, p.row_tiles * p.kv_heads, sequences), THREADS, bytes, stream, p);
+    launch_kernel(draft_attention_kernel<T, DMAX, PIECES>, dim3(p.shares, p.row_tiles * p.kv_heads, sequences), groups<T, DMAX>() * THREADS, bytes, stream, p);
     return check_launch("draft_attention");
 }
 template <typename T, bool PIECES>

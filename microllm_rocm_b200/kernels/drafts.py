@@ -20,7 +20,7 @@ from .device import sm_count
 
 MAX_NODES = 256             # csrc/drafts.cu: nodes of a sequence
 ROWS, KEYS = 16, 32         # csrc/drafts.cu: rows (node, head of a group) and keys a CTA works on at a time
-SHARE_KEYS = 64             # keys below which a share is not cut further
+SHARE_KEYS = 128            # keys below which a share is not cut further: a tile for each group of a CTA
 TC_HEAD_DIMS, TC_KEYS, TC_ROWS = (64, 128), 128, 128        # csrc/drafts_tc.cu: keys a tile, rows of a stream (a CTA has two)
 TC_STRETCH = 2              # units (row tile x key tile) a CTA takes at least: a turn of both streams
 
