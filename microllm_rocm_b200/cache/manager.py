@@ -89,6 +89,7 @@ class CacheManager:
         self.kv_storage: Dict[str, torch.Tensor] = {}
         self.state_storage: Dict[str, torch.Tensor] = {}
         self.state_needs: Dict[str, FixedStateNeed] = {}
+        self.paged_needs: Dict[str, object] = {}
         self.guarded: Dict[str, torch.Tensor] = {}       # entry -> the whole allocation, guards included
         for name, need in entries.items():
             need = getattr(need, "need", need)
@@ -97,6 +98,7 @@ class CacheManager:
                 if key not in self.groups:
                     self.groups[key] = CacheGroup(key, need.window, self.pages_for_group(need.window, max_step_tokens, kept_tokens(need)), kept_tokens(need))
                 self.entry_group[name] = key
+                self.paged_needs[name] = need
                 if device is not None:
                     pages = self.groups[key].pool.num_pages + 1        # the pool's pages, then the spare page (see pad_page)
                     whole = torch.zeros((pages + (2 if guard_pages else 0), *page_shape(need, page_size)),
@@ -122,6 +124,7 @@ class CacheManager:
         self.requests: Dict[Hashable, _Request] = {}
         self.pages_released_by_window = 0
         self.tables_version = 0          # grows whenever any block table changes: lets a reader skip a comparison
+        self._moves: Dict[str, object] = {}      # what page_moves and slot_moves made
 
     def pages_for_group(self, window: Optional[int], max_step_tokens: Optional[int], keep_first: int = 0) -> int:
         """Pages of a group's pool: num_pages for all keys; for a window, what max_requests requests can hold at
@@ -228,6 +231,27 @@ class CacheManager:
         if name in self.entry_group:
             return PagedKVView(self.kv_storage[name], block_table, self.page_size, True)
         return StateView(self.state_storage[name], slots, list(slots_host or []), True)
+
+    # ----- moving what requests hold (kernels/cache_moves.py) --------------------------------
+    def page_moves(self, group: str):
+        """The pools of a group's layers, for kernels that move tokens between pages in all of them at once."""
+        if group not in self._moves:
+            from ..kernels.cache_moves import PageMoves
+            storages = []
+            for name, of in self.entry_group.items():
+                if of == group:
+                    need, pool = self.paged_needs[name], self.kv_storage[name]
+                    widths = (need.num_kv_heads, need.head_dim, need.value_dim) if pool.dim() == 2 else None
+                    storages.append((pool, widths) if widths else pool)
+            self._moves[group] = PageMoves(storages, self.page_size)
+        return self._moves[group]
+
+    def slot_moves(self):
+        """The storages of fixed-size state, for kernels that move requests' state between slots in all of them at once."""
+        if "slots" not in self._moves:
+            from ..kernels.cache_moves import SlotMoves
+            self._moves["slots"] = SlotMoves([t.view(t.shape[0], -1) for t in self.state_storage.values()])
+        return self._moves["slots"]
 
     # ----- accounting and self-check -------------------------------------------------------
     def stats(self) -> Dict[str, object]:

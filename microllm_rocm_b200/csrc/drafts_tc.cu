@@ -61,10 +61,7 @@ constexpr int MAX_PAGES_PER_TILE = 16;
 constexpr int MAX_WORDS = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RESCALE_STEP = 8.0f;
-#ifndef V_CHUNK
-#define V_CHUNK 32
-#endif
-constexpr int CHUNK = V_CHUNK;
+constexpr int CHUNK = 32;                    // scores that a softmax thread has in registers at a time
 
 struct TcParams {
     __nv_bfloat16* out;             // [T, NH * D]
@@ -736,8 +733,7 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                         for (int i = 0; i < CHUNK / 32; ++i) tmem_ld32(tmem + (uint32_t)(c * CHUNK + i * 32), sr + i * 32);
                         tmem_wait_ld();
                         l += row_exp2(sr, p.scale_log2, shift);
-                        if constexpr (CHUNK == 64) tmem_st32(tmem + (uint32_t)(c * 32), sr);
-                        else tmem_st16(tmem + (uint32_t)(c * 16), sr);
+                        tmem_st16(tmem + (uint32_t)(c * (CHUNK / 2)), sr);
                     }
                     tmem_wait_st();
                 }
@@ -898,7 +894,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) draft_join_tc_kernel(TcParams p)
     if (parts == 1) return;                               // written whole
     const bool mine = lane < rows;
     float top = -INFINITY, sum = 0.0f, acc[COLS] = {};
-#pragma unroll 4
+#pragma unroll 2
     for (int k = SPREAD ? warp : 0; k < parts; k += SPREAD ? JOIN_WARPS : 1) {
         // part k lies with CTA first + k: the first part is of the item that its stretch ends in, the others of the one that it begins in; a part
         // may be no tile's

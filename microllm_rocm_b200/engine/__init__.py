@@ -1,1 +1,2 @@
 from .step import Engine, StepEntry, StepError, OutOfPages
+from .continuations import Accepted, DraftEntry, DraftStep

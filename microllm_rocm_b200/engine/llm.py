@@ -320,6 +320,12 @@ class LLM:
 
     generate_batch = generate
 
+    def beam_search(self, prompt: Sequence[int], num_beams: int = 4, max_new_tokens: int = 32, end_token: Optional[int] = None):
+        """The best continuations of `prompt` that a search with `num_beams` beams finds, by the sum of log probabilities: a list of (tokens, score), best first
+        (engine/continuations.py).  Runs at once, beside requests that the scheduler holds; it needs free pages and slots for its beams."""
+        from .continuations import beam_search
+        return beam_search(self.engine, prompt, num_beams, max_new_tokens, end_token)
+
     def metrics(self) -> Dict[str, object]:
         m = dict(vars(self.scheduler.metrics))
         m["cache"] = self.engine.cache.stats()

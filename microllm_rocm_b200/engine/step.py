@@ -209,6 +209,17 @@ class Engine:
         self.tokens_run += ctx.num_tokens
         return logits
 
+    def draft_step(self, entries):
+        """A step that brings a tree of drafted tokens per request (engine/continuations.py: DraftEntry); returns the logits of every node.  The
+        requests keep their lengths until `accept_drafts`."""
+        from .continuations import draft_step
+        return draft_step(self, entries)
+
+    def accept_drafts(self, step, choices: torch.Tensor):
+        """Keep the branch of each tree of a draft step that `choices` (the model's own token behind every node, [nodes] int32) confirm."""
+        from .continuations import accept_drafts
+        return accept_drafts(self, step, choices)
+
     def cache_views(self, ctx: StepContext) -> Dict[str, object]:
         cache = self.cache
         views = {}

@@ -9,7 +9,7 @@ the sequence's pages (`places`), while its position, which the rotation takes, i
 from __future__ import annotations
 
 from ctypes import c_float, c_int, c_void_p
-from typing import Optional
+from typing import Callable, Optional
 
 import torch
 
@@ -100,14 +100,16 @@ def _ctas(heads: int, row_tiles: int, key_tiles: int, sms: int) -> int:
 
 def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor,
                     masks: torch.Tensor, block_table: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, scale: float,
-                    window: Optional[int] = None, *, max_nodes: int, max_length: int, error_flag: Optional[torch.Tensor] = None) -> None:
+                    window: Optional[int] = None, *, max_nodes: int, max_length: int, error_flag: Optional[torch.Tensor] = None,
+                    alloc: Optional[Callable[[int], torch.Tensor]] = None) -> None:
     """out[t, h] = softmax(scale q[t, h] . k) v over what node t sees: its sequence's cached tokens and the nodes of its mask, of both only
     those of the last `window` positions where one is given.  A node that sees nothing gets zeros.
 
     `q` and `out` [T, heads * D], `pages` [pages, 2, kv heads, page, D] of the same type (fp32 or bf16); `positions` and `masks` as `draft_masks`
     makes them (any other mask over a sequence's nodes will do); `block_table` [sequences, blocks] int32.
     `max_nodes`: the most nodes of a sequence, which the launch is sized for (a sequence of more raises the error flag).  `max_length`: the most keys
-    of a sequence, its nodes among them (how the work is cut; a longer sequence costs time only)."""
+    of a sequence, its nodes among them (how the work is cut; a longer sequence costs time only).  `alloc(bytes)` -> uint8 tensor: the step's own memory
+    for partial results, for a caller whose launches are recorded and issued again; else it is taken and given back in the current stream's order."""
     device = q.get_device()
     tag, dtype = ops.dtype_tag(q), q.dtype
     need_on(device, (q, "q", dtype, 2), (pages, "pages", dtype, 5), (out, "out", dtype, 2), (positions, "positions", INT, 1), (masks, "masks", INT, 2),
@@ -131,12 +133,13 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     if T == 0 or sequences == 0:
         return
     need_current(device, "draft_attention")
+    alloc = alloc or (lambda nbytes: ops.scratch(nbytes, q.device, "draft_attention"))
     group = num_heads // num_kv_heads
     q_at, pages_at, out_at = q.data_ptr(), pages.data_ptr(), out.data_ptr()
     if dtype is torch.bfloat16 and tc_supported(head_dim, page_size, group, scale) and not (q_at | pages_at | out_at) & 15:
         keys = min(max_length, window + max_nodes + TC_KEYS) if window else max_length
         ctas = _ctas(sequences * num_kv_heads, -(-max_nodes // (TC_ROWS // group)), -(-keys // TC_KEYS), _sm_count(device))
-        scratch = ops.scratch(ctas * 4 * TC_ROWS * (head_dim + 2) * 4 + 8 + 4 * sequences, q.device, "draft_attention") if ctas > 1 else None
+        scratch = alloc(ctas * 4 * TC_ROWS * (head_dim + 2) * 4 + 8 + 4 * sequences) if ctas > 1 else None
         L = ops.lib("drafts_tc.cu", _TC_DEFINES[head_dim])
         build.check(L, L.mlb_draft_attention_tc(q_at, pages_at, out_at, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
                                                 masks.data_ptr(), words, block_table.data_ptr(), block_table.shape[1], num_pages, page_size, T, sequences,
@@ -146,7 +149,7 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     keys = min(max_length, window + max_nodes + KEYS) if window else max_length
     row_tiles = -(-max_nodes * group // ROWS)
     share, shares = _shares(sequences * num_kv_heads * row_tiles, keys, _sm_count(device))
-    scratch = ops.scratch(shares * T * num_heads * (head_dim + 2) * 4, q.device, "draft_attention") if shares > 1 else None
+    scratch = alloc(shares * T * num_heads * (head_dim + 2) * 4) if shares > 1 else None
     L = ops.lib("drafts.cu")
     build.check(L, L.mlb_draft_attention(q_at, pages_at, out_at, tag, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
                                          masks.data_ptr(), words, block_table.data_ptr(), block_table.shape[1], num_pages, page_size, T, sequences, int(max_nodes),

@@ -63,6 +63,8 @@ class Attention(Mixer):
         if self.rotary is None:        # no rotation: an empty table makes the kernel pass q/k through
             self._no_rot = torch.zeros(0, dtype=torch.float32, device=rt.device)
         self.w_qkv = self.b_qkv = self.w_o = self.b_o = None
+        # a drafted tree's tokens are rotated by one number and stored by another: where the rotation takes the step's table of angles
+        self.takes_drafts = self.rotary is None or (self.rotary.rotary_dim == self.d and not self.rotary.interleaved and self.d % 16 == 0)
 
     # --- declarations -----------------------------------------------------------------
     def cache_need(self):
@@ -135,7 +137,7 @@ class Attention(Mixer):
         inv_freq, rot, inter = ((self.rotary.inv_freq, self.rotary.rotary_dim, self.rotary.interleaved)
                                 if self.rotary is not None else (self._no_rot, 0, False))
         pages = cache.pages if cache.writable else None
-        if (x.dtype == torch.bfloat16 and gemm_bf16.gemv_preferred(x, self.w_qkv)
+        if ctx.tree is None and (x.dtype == torch.bfloat16 and gemm_bf16.gemv_preferred(x, self.w_qkv)
                 and gemm_bf16.gemv_fused_supported(x, self.w_qkv) and self.d % 16 == 0
                 and (rot == 0 or (rot == self.d and not inter))):
             # a few tokens: projection, bias, rotation and the cache store in one weight-streaming kernel
@@ -145,7 +147,7 @@ class Attention(Mixer):
             qkv = linear(x, self.w_qkv, None, torch.float32, partials_ok=True,    # [T, (NH+2NKV)*D] f32, or its partial sums
                          alloc=lambda shape, dtype: ctx.buffer("attention.qkv", shape, dtype), error_flag=ctx.error_flag)
             cos_sin = None
-            if rot and T >= ROPE_TABLE_MIN_TOKENS and x.dtype == torch.bfloat16:
+            if rot and (ctx.tree is not None or T >= ROPE_TABLE_MIN_TOKENS and x.dtype == torch.bfloat16):
                 # a prompt portion: the step's sines and cosines are made once and serve every layer and head
                 # (a result of this step's positions: it lives in step_values, which every forward starts empty,
                 # so a context that outlives its step -- a captured decode step -- never reads old angles)
@@ -154,12 +156,19 @@ class Attention(Mixer):
                 if cos_sin is None:
                     table = ctx.buffer("attention.rope_table", (T, rot // 2, 2), torch.float32)
                     cos_sin = ctx.step_values[key] = ops.rope_table(ctx.positions, inv_freq, out=table)
-            ops.rope_kv_write(qkv, self.b_qkv, ctx.positions, ctx.token_seq, cache.block_table, inv_freq, rot, inter,
+            ops.rope_kv_write(qkv, self.b_qkv, ctx.positions if ctx.tree is None else ctx.places, ctx.token_seq, cache.block_table, inv_freq, rot, inter,
                               q, pages, self.nh, self.nkv, self.d, ctx.error_flag, cos_sin)
         o = ctx.buffer("attention.o", (T, self.nh * self.d), self.rt.dtype)
-        attention_kernels.paged_attention(q, cache.pages, o, ctx, cache.block_table, self.nh, self.nkv, self.d,
-                                          self.scale, self.window,
-                                          beside_mma_products=x.dtype == torch.bfloat16 and gemm_bf16.gemv_preferred(x, self.w_o))
+        if ctx.tree is not None:
+            from ..kernels import drafts
+            masks, _, most = ctx.tree
+            drafts.draft_attention(q, cache.pages, o, ctx.seq_starts, ctx.seq_pos0, ctx.positions, masks, cache.block_table, self.nh, self.nkv, self.d,
+                                   self.scale, self.window, max_nodes=most, max_length=ctx.max_seq_len, error_flag=ctx.error_flag,
+                                   alloc=lambda nbytes: ctx.buffer("attention.drafts", (nbytes,), torch.uint8))
+        else:
+            attention_kernels.paged_attention(q, cache.pages, o, ctx, cache.block_table, self.nh, self.nkv, self.d,
+                                              self.scale, self.window,
+                                              beside_mma_products=x.dtype == torch.bfloat16 and gemm_bf16.gemv_preferred(x, self.w_o))
         return linear(o, self.w_o, self.b_o, torch.float32, partials_ok=True, error_flag=ctx.error_flag,      # [T, H] f32, or its partial sums
                       alloc=lambda shape, dtype: ctx.buffer("attention.out", shape, dtype))
 

@@ -162,6 +162,10 @@ class StepContext:
     # tensor trace.  Such a step runs every layer call by call.
     tensor_sink: Optional[Callable[[str, torch.Tensor], None]] = None
     mean_seq_len: float = 0.0      # mean length of the sequences after the step (0: not known, taken for the longest)
+    # A step whose sequences bring trees of drafted tokens instead of runs of them: (masks [T, words], parents [T], the most nodes of a sequence); then
+    # `positions` says how deep a token lies, and `places` [T] where its key and value go (places lie side by side, positions repeat)
+    tree: Optional[Tuple[torch.Tensor, torch.Tensor, int]] = None
+    places: Optional[torch.Tensor] = None
     captured: bool = False         # its launches are recorded and run again, by whichever thread: nothing of theirs may be a thread's own
 
     @property
@@ -265,6 +269,8 @@ class Mixer(Part):
     # inputs (no host mirrors of the context, no synchronisation): such a mixer may be
     # captured into a CUDA graph for steady decoding.
     graph_safe = False
+    # True when forward() takes steps with a `tree` (StepContext.tree).
+    takes_drafts = False
 
     def cache_need(self):
         """PagedKVNeed, FixedStateNeed or None."""
