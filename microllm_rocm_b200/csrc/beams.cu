@@ -187,9 +187,9 @@ template <> struct Row<__nv_bfloat16> {
     }
 };
 
-__device__ __forceinline__ float max_nan(float a, float b) {       // NaN where either is
+__device__ __forceinline__ float max_nan(float a, float b, float c) {       // NaN where one of them is
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -197,6 +197,11 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));      // (what is below 2^-126 adds nothing to a sum that is at least 1)
     return r;
 }
+
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) { return ((f32x2)__float_as_uint(hi) << 32) | __float_as_uint(lo); }
+__device__ __forceinline__ float low(f32x2 v) { return __uint_as_float((unsigned)v); }
+__device__ __forceinline__ float high(f32x2 v) { return __uint_as_float((unsigned)(v >> 32)); }
 
 // Logits whose product with log2 e is none (a mask of the type's lowest value on a whole row): their differences are taken first.
 __device__ __forceinline__ bool is_far(float top) { return fabsf(top) > 1e37f; }
@@ -228,13 +233,21 @@ __global__ void __launch_bounds__(THREADS, 4) select_slices_kernel(SelectParams 
     auto place_of = [&](int count) { return count > THREADS * W ? tid : lane * WARPS + warp; };
     extern __shared__ __align__(16) unsigned char next_s[];
     uint4* const next = reinterpret_cast<uint4*>(next_s) + tid;       // piece k: next[k * THREADS]
+    const unsigned next_at = (unsigned)__cvta_generic_to_shared(next);
     auto ask = [&](int from) {
         const int count = min(SLICE, end - from), place = place_of(count);
+        if (count == SLICE) {
+            const T* const at = x + from + tid * W;
 #pragma unroll
+            for (int k = 0; k < PIECES; ++k)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(next_at + k * THREADS * 16), "l"(at + k * THREADS * W) : "memory");
+            return;
+        }
+#pragma unroll 1
         for (int k = 0; k < PIECES; ++k) {
             const int i = (k * THREADS + place) * W, there = min(W, count - i);
             if (there > 0)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((unsigned)__cvta_generic_to_shared(next + k * THREADS)), "l"(x + from + i),
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(next_at + k * THREADS * 16), "l"(x + from + i),
                              "r"(there * (int)sizeof(T)) : "memory");
         }
     };
@@ -266,10 +279,14 @@ __global__ void __launch_bounds__(THREADS, 4) select_slices_kernel(SelectParams 
             const int i = (k / W * THREADS + place) * W + k % W;
             return i < count ? to_f32(x[from + i]) : -INFINITY;
         };
-        float most[4] = {v[0], v[1], v[2], v[3]};
+        // groups of eight neighbours, and their largest
+        float most[4];
 #pragma unroll
-        for (int k = 4; k < PER; ++k) most[k & 3] = max_nan(most[k & 3], v[k]);
-        const float mine = max_nan(max_nan(most[0], most[1]), max_nan(most[2], most[3]));
+        for (int g = 0; g < 4; ++g) {
+            const float* const u = v + g * 8;
+            most[g] = max_nan(max_nan(u[0], u[1], u[2]), max_nan(u[3], u[4], u[5]), max_nan(u[6], u[7], u[7]));
+        }
+        const float mine = max_nan(max_nan(most[0], most[1], most[2]), most[3], most[3]);
         bad |= !(mine < INFINITY);
         if (mine > top) {
             const float new_top2 = mine * LOG2E;
@@ -278,15 +295,25 @@ __global__ void __launch_bounds__(THREADS, 4) select_slices_kernel(SelectParams 
             top2 = new_top2;
         }
         if (top > -INFINITY) {
-            float part_sum[2] = {0.0f, 0.0f};
+            float part_sum;
             if (is_far(top)) {
+                part_sum = 0.0f;
 #pragma unroll 1
-                for (int k = 0; k < PER; ++k) part_sum[0] += exp2_approx((at_of(k) - top) * LOG2E);
+                for (int k = 0; k < PER; ++k) part_sum += exp2_approx((at_of(k) - top) * LOG2E);
             } else {
+                // two to an instruction, each rounded as always
+                const f32x2 scale = pair(LOG2E, LOG2E), shift = pair(-top2, -top2);
+                f32x2 sums = 0ull;
 #pragma unroll
-                for (int k = 0; k < PER; ++k) part_sum[k & 1] += exp2_approx(fmaf(v[k], LOG2E, -top2));
+                for (int k = 0; k < PER; k += 2) {
+                    f32x2 e;
+                    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e) : "l"(pair(v[k], v[k + 1])), "l"(scale), "l"(shift));
+                    e = pair(exp2_approx(low(e)), exp2_approx(high(e)));
+                    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sums) : "l"(e));
+                }
+                part_sum = low(sums) + high(sums);
             }
-            sum += (double)(part_sum[0] + part_sum[1]);
+            sum += (double)part_sum;
         }
         float least = bound;
         if (bound == -FLT_MAX) {                  // (the same in all threads) no slice so far had `wanted` elements
@@ -303,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, 4) select_slices_kernel(SelectParams 
         for (int g = 0; g < 4; ++g) {
             if (!__any_sync(0xffffffffu, most[g] >= least)) continue;
 #pragma unroll
-            for (int k = g; k < PER; k += 4)
+            for (int k = g * 8; k < g * 8 + 8; ++k)
                 if (v[k] >= least) {
                     const int to = atomicAdd(&s.count, 1);
                     if (to < LIST) { s.value[to] = v[k]; s.index[to] = from + (k / W * THREADS + place) * W + k % W; }
