@@ -14,6 +14,7 @@
 #include <cfloat>
 
 #include "common.cuh"
+#include "packed.cuh"
 
 using namespace mlb;
 
@@ -564,3 +565,5 @@ MLB_EXPORT int mlb_beam_select(const void* logits, int dtype, long long ld, cons
     launch_kernel(select_join_kernel, requests, THREADS, 0, stream, p);
     return check_launch("beam_select join");
 }
+
+MLB_PACKED(mlb_beam_select)

@@ -7,6 +7,7 @@
 // needs neither a scratch copy nor a synchronisation, and what bounds the kernels is memory: each moved destination is written
 // once, each source read once from memory (children of one parent read it from the L1 of the same thread).
 #include "common.cuh"
+#include "packed.cuh"
 
 using namespace mlb;
 
@@ -394,3 +395,7 @@ MLB_EXPORT int mlb_accept_drafts(const void* const* bases, int count, long long 
 }
 
 MLB_EXPORT int mlb_moves_max_storages() { return MAX_STORAGES; }
+
+MLB_PACKED(mlb_reorder_slots)
+MLB_PACKED(mlb_reorder_pages)
+MLB_PACKED(mlb_accept_drafts)

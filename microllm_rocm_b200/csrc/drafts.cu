@@ -11,6 +11,7 @@
 //
 // The tensor-core kernel for bf16 heads of 64 and 128 is csrc/drafts_tc.cu.
 #include "common.cuh"
+#include "packed.cuh"
 
 using namespace mlb;
 
@@ -419,3 +420,6 @@ MLB_EXPORT int mlb_draft_attention(const void* q, const void* pages, void* out, 
     if (dtype == MLB_BF16) return run_attention<__nv_bfloat16>(p, sequences, max_nodes, stream);
     return fail(MLB_INVALID_ARGUMENT, "draft_attention: fp32 or bf16");
 }
+
+MLB_PACKED(mlb_draft_masks)
+MLB_PACKED(mlb_draft_attention)

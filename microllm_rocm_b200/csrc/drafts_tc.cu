@@ -24,6 +24,7 @@
 // Every wait on an mbarrier is bounded; when a bound is hit the error flag is raised, the CTA waits (bounded) for the copies in flight, frees
 // its tensor memory and returns.
 #include "common.cuh"
+#include "packed.cuh"
 
 #include <cuda.h>
 
@@ -1042,3 +1043,5 @@ MLB_EXPORT int mlb_draft_attention_tc(const void* q, const void* pages, void* ou
     else launch_kernel(draft_join_tc_kernel<false>, dim3(blocks, sequences), JOIN_THREADS, 0, stream, p);
     return check_launch("draft_join_tc");
 }
+
+MLB_PACKED(mlb_draft_attention_tc)

@@ -102,6 +102,10 @@ def need_on(device_index: int, *tensors) -> None:
             raise KernelError(f"{name} must be a contiguous {dtype} tensor of {dims} dimensions on the call's device, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
+def _address(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def need_current(device_index: int, what: str) -> None:
     """Launches go to the current device's stream: the tensors have to lie there."""
     if device_index < 0:
@@ -137,7 +141,7 @@ def reorder_slots(moves: SlotMoves, slots: torch.Tensor, parents: torch.Tensor, 
     need_current(device, "reorder_slots")
     L = ops.lib("cache_moves.cu")
     for address, count, layout, _ in moves.groups:
-        build.check(L, L.mlb_reorder_slots(address, count, *layout, slots.data_ptr(), parents.data_ptr(), requests, beams, ops._ptr(error_flag), ops._stream()))
+        build.check(L, L.mlb_reorder_slots(address, count, *layout, slots.data_ptr(), parents.data_ptr(), requests, beams, _address(error_flag), ops._stream()))
 
 
 def reorder_pages(moves: PageMoves, block_table: torch.Tensor, parents: torch.Tensor, first: torch.Tensor, last: torch.Tensor, max_tokens: int,
@@ -166,4 +170,4 @@ def reorder_pages(moves: PageMoves, block_table: torch.Tensor, parents: torch.Te
     L = ops.lib("cache_moves.cu")
     for address, count, layout, _ in moves.groups:
         build.check(L, L.mlb_reorder_pages(address, count, *layout, block_table.data_ptr(), block_table.shape[1], parents.data_ptr(), requests, beams,
-                                           first.data_ptr(), last.data_ptr(), int(max_tokens), ops._ptr(error_flag), ops._stream()))
+                                           first.data_ptr(), last.data_ptr(), int(max_tokens), _address(error_flag), ops._stream()))

@@ -15,7 +15,7 @@ import torch
 
 from . import build, ops
 from .build import KernelError
-from .cache_moves import INT, PageMoves, need_current, need_on
+from .cache_moves import INT, PageMoves, _address, need_current, need_on
 from .device import sm_count
 
 MAX_NODES = 256             # csrc/drafts.cu: nodes of a sequence
@@ -83,7 +83,7 @@ def draft_masks(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tens
     need_current(device, "draft_masks")
     L = ops.lib("drafts.cu")
     build.check(L, L.mlb_draft_masks(parents.data_ptr(), starts.data_ptr(), lengths.data_ptr(), sequences, masks.shape[1], masks.data_ptr(), positions.data_ptr(),
-                                     ops._ptr(places), ops._ptr(error_flag), ops._stream()))
+                                     _address(places), _address(error_flag), ops._stream()))
 
 
 def _shares(ctas: int, keys: int, sms: int):
@@ -96,6 +96,10 @@ def _shares(ctas: int, keys: int, sms: int):
 def _ctas(heads: int, row_tiles: int, key_tiles: int, sms: int) -> int:
     """CTAs of the tensor-core kernel: one a multiprocessor, as long as each finds TC_STRETCH units of heads x row tiles x key tiles."""
     return max(1, min(sms, -(-heads * row_tiles * key_tiles // TC_STRETCH)))
+
+
+def _memory(alloc, q: torch.Tensor, nbytes: int) -> torch.Tensor:
+    return ops.scratch(nbytes, q.device, "draft_attention") if alloc is None else alloc(nbytes)
 
 
 def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor,
@@ -113,17 +117,16 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     device = q.get_device()
     tag, dtype = ops.dtype_tag(q), q.dtype
     need_on(device, (q, "q", dtype, 2), (pages, "pages", dtype, 5), (out, "out", dtype, 2), (positions, "positions", INT, 1), (masks, "masks", INT, 2),
-            (block_table, "block_table", INT, 2))
-    sequences = _need_trees(device, starts, lengths)
-    T, width = q.shape
+            (block_table, "block_table", INT, 2), (starts, "starts", INT, 1), (lengths, "lengths", INT, 1))
+    (T, width), (rows, words), (sequences, max_blocks) = q.shape, masks.shape, block_table.shape
     num_pages, two, nkv, page_size, d = pages.shape
     if two != 2 or nkv != num_kv_heads or d != head_dim:
         raise KernelError(f"draft_attention: pages {tuple(pages.shape)} do not match the head geometry")
     if num_kv_heads <= 0 or num_heads % num_kv_heads or not 0 < head_dim <= 256:
         raise KernelError(f"draft_attention: heads {num_heads}/{num_kv_heads} of {head_dim}")
-    if width != num_heads * head_dim or out.shape != q.shape or positions.shape[0] != T or masks.shape[0] != T or block_table.shape[0] != sequences:
+    if (width != num_heads * head_dim or rows != T or out.shape != q.shape or positions.shape[0] != T or lengths.shape[0] != sequences
+            or starts.shape[0] != sequences + 1):
         raise KernelError("draft_attention: shapes do not agree")
-    words = masks.shape[1]
     if not 0 < words <= MAX_NODES // 32 or not 0 < max_nodes <= words * 32 or max_length < max_nodes:
         raise KernelError(f"draft_attention: {max_nodes} nodes among {max_length} keys in masks of {words} words (at most {MAX_NODES // 32})")
     if window is not None and window <= 0:
@@ -133,28 +136,27 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     if T == 0 or sequences == 0:
         return
     need_current(device, "draft_attention")
-    alloc = alloc or (lambda nbytes: ops.scratch(nbytes, q.device, "draft_attention"))
     group = num_heads // num_kv_heads
     q_at, pages_at, out_at = q.data_ptr(), pages.data_ptr(), out.data_ptr()
     if dtype is torch.bfloat16 and tc_supported(head_dim, page_size, group, scale) and not (q_at | pages_at | out_at) & 15:
         keys = min(max_length, window + max_nodes + TC_KEYS) if window else max_length
         ctas = _ctas(sequences * num_kv_heads, -(-max_nodes // (TC_ROWS // group)), -(-keys // TC_KEYS), _sm_count(device))
-        scratch = alloc(ctas * 4 * TC_ROWS * (head_dim + 2) * 4 + 8 + 4 * sequences) if ctas > 1 else None
+        scratch = _memory(alloc, q, ctas * 4 * TC_ROWS * (head_dim + 2) * 4 + 8 + 4 * sequences) if ctas > 1 else None
         L = ops.lib("drafts_tc.cu", _TC_DEFINES[head_dim])
         build.check(L, L.mlb_draft_attention_tc(q_at, pages_at, out_at, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
-                                                masks.data_ptr(), words, block_table.data_ptr(), block_table.shape[1], num_pages, page_size, T, sequences,
-                                                int(max_nodes), num_heads, num_kv_heads, float(scale), int(window or 0), TC_STRETCH, ctas, ops._ptr(scratch),
-                                                ops._ptr(error_flag), ops._stream()))
+                                                masks.data_ptr(), words, block_table.data_ptr(), max_blocks, num_pages, page_size, T, sequences,
+                                                int(max_nodes), num_heads, num_kv_heads, float(scale), int(window or 0), TC_STRETCH, ctas, _address(scratch),
+                                                _address(error_flag), ops._stream()))
         return
     keys = min(max_length, window + max_nodes + KEYS) if window else max_length
     row_tiles = -(-max_nodes * group // ROWS)
     share, shares = _shares(sequences * num_kv_heads * row_tiles, keys, _sm_count(device))
-    scratch = alloc(shares * T * num_heads * (head_dim + 2) * 4) if shares > 1 else None
+    scratch = _memory(alloc, q, shares * T * num_heads * (head_dim + 2) * 4) if shares > 1 else None
     L = ops.lib("drafts.cu")
     build.check(L, L.mlb_draft_attention(q_at, pages_at, out_at, tag, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
-                                         masks.data_ptr(), words, block_table.data_ptr(), block_table.shape[1], num_pages, page_size, T, sequences, int(max_nodes),
-                                         num_heads, num_kv_heads, head_dim, float(scale), int(window or 0), share, shares, ops._ptr(scratch),
-                                         ops._ptr(error_flag), ops._stream()))
+                                         masks.data_ptr(), words, block_table.data_ptr(), max_blocks, num_pages, page_size, T, sequences, int(max_nodes),
+                                         num_heads, num_kv_heads, head_dim, float(scale), int(window or 0), share, shares, _address(scratch),
+                                         _address(error_flag), ops._stream()))
 
 
 def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor,
@@ -168,8 +170,8 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
     device = tokens.get_device()
     need_on(device, (tokens, "tokens", INT, 1), (parents, "parents", INT, 1), (choices, "choices", INT, 1), (path, "path", INT, 2), (counts, "counts", INT, 1),
             (following, "following", INT, 1))
-    sequences = _need_trees(device, starts, lengths)
-    if parents.shape != tokens.shape or choices.shape != tokens.shape:
+    sequences, T = _need_trees(device, starts, lengths), tokens.shape
+    if parents.shape != T or choices.shape != T:
         raise KernelError("accept_drafts: one token, parent and choice per node")
     if path.shape[0] != sequences or path.shape[1] == 0 or counts.shape[0] != sequences or following.shape[0] != sequences:
         raise KernelError("accept_drafts: one path, count and following token per sequence")
@@ -190,7 +192,7 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
     need_current(device, "accept_drafts")
     L = ops.lib("cache_moves.cu")
     trees = (tokens.data_ptr(), parents.data_ptr(), choices.data_ptr(), starts.data_ptr(), lengths.data_ptr(), sequences)
-    for i, (address, count, layout, _) in enumerate(groups or [(None, 0, (1, 1, 1, 1, 0, 0), None)]):
-        build.check(L, L.mlb_accept_drafts(address, count, *layout, *trees, ops._ptr(block_table), block_table.shape[1] if block_table is not None else 0,
+    for i, (address, count, layout, _) in enumerate(groups or [(0, 0, (1, 1, 1, 1, 0, 0), None)]):
+        build.check(L, L.mlb_accept_drafts(address, count, *layout, *trees, _address(block_table), block_table.shape[1] if block_table is not None else 0,
                                            path.data_ptr(), path.shape[1], counts.data_ptr(), following.data_ptr(), 1 if i == 0 else 0,
-                                           ops._ptr(error_flag), ops._stream()))
+                                           _address(error_flag), ops._stream()))

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import struct
 import threading
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from typing import Optional
@@ -160,6 +161,25 @@ def lagged_draft_sources():
     return [("drafts_tc.cu", {"HEAD_DIM": 128, "MLB_LAG_WARP": w}) for w in (0, 1, 5, 10)]
 
 
+_PACKED_FORMATS = {c_void_p: "P", c_int: "i", c_longlong: "q", c_float: "f"}
+
+
+class Packed:
+    """A launcher that takes its arguments in one block as well (csrc/packed.cuh), which is the shorter way unless a recorder wants to see them.  Null
+    pointers are 0."""
+    __slots__ = ("launcher", "function", "pack", "replay", "__name__")
+
+    def __init__(self, launcher, function, replay):
+        function.argtypes, function.restype = [c_void_p], c_int
+        self.launcher, self.function, self.replay, self.__name__ = launcher, function, replay, launcher.__name__
+        self.pack = struct.Struct("@" + "".join(_PACKED_FORMATS[t] for t in launcher.argtypes)).pack
+
+    def __call__(self, *args):
+        if self.replay._active is None:
+            return self.function(self.pack(*args))
+        return self.launcher(*args)
+
+
 def lib(source: str, defines=None) -> ctypes.CDLL:
     if TEST_DEFINES.get(source):
         defines = {**(defines or {}), **TEST_DEFINES[source]}
@@ -167,17 +187,20 @@ def lib(source: str, defines=None) -> ctypes.CDLL:
     got = _libs.get(key)
     if got is None:
         got = build.load(source, defines)
-        from .replay import Launcher
+        from . import replay
+        Launcher = replay.Launcher
         for name, argtypes in _SIGNATURES.get(source, {}).items():
             fn = getattr(got, name)
-            if isinstance(fn, Launcher):
+            if isinstance(fn, (Launcher, Packed)):
                 continue
             fn.argtypes = argtypes
             fn.restype = c_int
             if argtypes and argtypes[-1] is c_void_p:
                 # a launcher (its last argument is the stream): calls through; a recorder may listen (kernels/replay.py).
                 # Queries (split counts, limits) return numbers, not a status, and are never recorded.
-                setattr(got, name, Launcher(got, fn, argtypes))
+                launcher = Launcher(got, fn, argtypes)
+                packed = getattr(got, name + "_packed", None)
+                setattr(got, name, launcher if packed is None else Packed(launcher, packed, replay))
         _libs[key] = got
     return got
 
@@ -306,7 +329,6 @@ def activation_code(activation: str, limit: Optional[float] = None) -> int:
     """What the gated kernels take as `act`: 0 silu, 1 gelu_tanh; for the clamped form the bit pattern of its positive fp32
     limit (an int above 1 for every normal number), so that the limit travels in the same argument."""
     if activation == CLAMPED_ACTIVATION:
-        import struct
         if limit is None or not limit > 0:
             raise KernelError("the clamped activation needs a positive limit")
         code = struct.unpack("<i", struct.pack("<f", float(limit)))[0]
