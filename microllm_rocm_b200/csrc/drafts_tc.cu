@@ -204,43 +204,57 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&v);
 }
 
-// The largest of a row's scores: eight chains of three operands a step.
+// The largest of a row's scores, NaN where one is: eight chains of three operands a step.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {       // NaN where one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 template <int N>
 __device__ __forceinline__ float row_max(const uint32_t (&s)[N]) {
+    auto at = [&](int i) { return __uint_as_float(s[i]); };
     float m[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m[k] = fmaxf(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+    for (int k = 0; k < 8; ++k) m[k] = max_nan(at(2 * k), at(2 * k + 1), at(2 * k + 1));
 #pragma unroll
-    for (int c = 16; c < N; c += 2) m[(c >> 1) & 7] = fmaxf(fmaxf(m[(c >> 1) & 7], __uint_as_float(s[c])), __uint_as_float(s[c + 1]));
-    return fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), fmaxf(fmaxf(m[4], m[5]), fmaxf(m[6], m[7])));
+    for (int c = 16; c < N; c += 2) m[(c >> 1) & 7] = max_nan(m[(c >> 1) & 7], at(c), at(c + 1));
+    return max_nan(max_nan(m[0], m[1], m[2]), max_nan(m[3], m[4], m[5]), max_nan(m[6], m[7], m[7]));
 }
 
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) { return ((f32x2)__float_as_uint(hi) << 32) | __float_as_uint(lo); }
+__device__ __forceinline__ float low(f32x2 v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high(f32x2 v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 // P = 2^(s * scale + shift) of N of a row's scores, as bf16 pairs in s[0 .. N / 2); returns the sum of the fp32 terms: neighbours first, then four
 // chains of them.  Scaling and summing go two to an instruction, each rounded as always.
 template <int N>
 __device__ __forceinline__ float row_exp2(uint32_t (&s)[N], float scale, float shift) {
-    typedef unsigned long long f32x2;
-    auto pair = [](uint32_t lo, uint32_t hi) { return ((f32x2)hi << 32) | lo; };
-    const f32x2 scale2 = pair(__float_as_uint(scale), __float_as_uint(scale)), shift2 = pair(__float_as_uint(shift), __float_as_uint(shift));
+    const f32x2 scale2 = pair(scale, scale), shift2 = pair(shift, shift);
     f32x2 chains[2] = {0ull, 0ull};          // chains 0 and 1, 2 and 3
 #pragma unroll
     for (int c = 0; c < N; c += 4) {
         float p[4];
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-            f32x2 x;
-            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(x) : "l"(pair(s[c + i], s[c + i + 1])), "l"(scale2), "l"(shift2));
-            p[i] = fast_exp2(__uint_as_float((uint32_t)x));
-            p[i + 1] = fast_exp2(__uint_as_float((uint32_t)(x >> 32)));
+            const f32x2 x = fma2(pair(__uint_as_float(s[c + i]), __uint_as_float(s[c + i + 1])), scale2, shift2);
+            p[i] = fast_exp2(low(x));
+            p[i + 1] = fast_exp2(high(x));
         }
-        f32x2 neighbours;
-        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(neighbours) : "l"(pair(__float_as_uint(p[0]), __float_as_uint(p[2]))), "l"(pair(__float_as_uint(p[1]), __float_as_uint(p[3]))));
-        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(chains[(c >> 2) & 1]) : "l"(neighbours));
+        chains[(c >> 2) & 1] = add2(chains[(c >> 2) & 1], add2(pair(p[0], p[2]), pair(p[1], p[3])));
         s[c / 2] = pack_bf16(p[0], p[1]);
         s[c / 2 + 1] = pack_bf16(p[2], p[3]);
     }
-    auto sum = [](f32x2 v) { return __uint_as_float((uint32_t)v) + __uint_as_float((uint32_t)(v >> 32)); };
-    return sum(chains[0]) + sum(chains[1]);
+    return (low(chains[0]) + high(chains[0])) + (low(chains[1]) + high(chains[1]));
 }
 
 
@@ -555,10 +569,12 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                 auto issue_qk = [&](int s, int i, bool last_use, bool last) {       // stream s's scores from ring item i
                     const uint32_t kb = ring_s + (i % SLOTS) * KV_BYTES, qb = q_s + (paired ? s * Q_BYTES : 0);
                     if (elect_one()) {
+                        // (a descriptor's address counts 16 bytes, so the next step's is a sum: made anew each time it cost as long as the product ran)
+                        const uint64_t qd = desc_k_major(qb), kd = desc_k_major(kb);
 #pragma unroll
                         for (int ks = 0; ks < D / 16; ++ks) {
-                            const uint32_t off = (ks / 4) * (BM * ROW_BYTES) + (ks % 4) * 32;
-                            umma(tmem_base + (uint32_t)(s * STREAM_COLS), desc_k_major(qb + off), desc_k_major(kb + off), idesc_qk, ks > 0);
+                            const uint32_t off = ((ks / 4) * (BM * ROW_BYTES) + (ks % 4) * 32) >> 4;
+                            umma(tmem_base + (uint32_t)(s * STREAM_COLS), qd + off, kd + off, idesc_qk, ks > 0);
                         }
                         if (last_use) umma_commit(smem_u32(&sh.slot_empty[i % SLOTS]));
                         if (last) umma_commit(smem_u32(&sh.q_empty));
@@ -569,10 +585,11 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                 auto issue_pv = [&](int s, int i, bool first, bool last, bool last_use) {
                     const uint32_t vb = ring_s + (i % SLOTS) * KV_BYTES;
                     if (elect_one()) {
+                        const uint64_t vd = desc_mn_major(vb, BN * ROW_BYTES);
 #pragma unroll
                         for (int ks = 0; ks < BN / 16; ++ks)           // 16 keys = 8 columns of P
                             umma_ts(tmem_base + (uint32_t)(s * STREAM_COLS + O_COL), tmem_base + (uint32_t)(s * STREAM_COLS + ks * 8),
-                                    desc_mn_major(vb + ks * 16 * ROW_BYTES, BN * ROW_BYTES), idesc_pv, (!first || ks > 0) ? 1u : 0u);
+                                    vd + ((ks * 16 * ROW_BYTES) >> 4), idesc_pv, (!first || ks > 0) ? 1u : 0u);
                         if (last_use) umma_commit(smem_u32(&sh.slot_empty[i % SLOTS]));
                         if (last) umma_commit(smem_u32(&sh.o_full[s]));
                     }
@@ -597,16 +614,13 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                     lag_point();
                     const bool more = t + dt < n_tiles, last = t + dt >= n_tiles;
                     const int s0 = paired ? 0 : t & 1;
-                    ok = wait_warp(&sh.p_full[s0], turn[s0] & 1, 45) && full(item, 46);
+                    // (the tiles first: they are there long before P, and each look at a barrier costs a hundred cycles of the way from P to the next scores)
+                    ok = full(item, 46) && (!more || full(item + 1, 47)) && wait_warp(&sh.p_full[s0], turn[s0] & 1, 45);
                     if (!ok) break;
                     ++turn[s0];
                     tc_fence_after();
                     issue_pv(s0, item, t < dt, last, !paired);
-                    if (more) {
-                        ok = full(item + 1, 47);
-                        if (!ok) break;
-                        issue_qk(s0, item + 1, !paired, !paired && t + dt + 1 == n_tiles);
-                    }
+                    if (more) issue_qk(s0, item + 1, !paired, !paired && t + dt + 1 == n_tiles);
                     if (paired) {
                         ok = wait_warp(&sh.p_full[1], turn[1] & 1, 48);
                         if (!ok) break;
@@ -707,9 +721,11 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                                 tmem_st32(tmem + (uint32_t)(c * CHUNK + i * 32), sr + i * 32);
                             }
                         }
-                        top = fmaxf(top, row_max(sr));
+                        top = max_nan(top, row_max(sr), top);
                     }
                     if (edge) tmem_wait_st();
+                    // a score that is NaN or +inf: the row becomes NaN (fmaxf passes over a NaN)
+                    if (!(top < INFINITY)) { sees_odd = true; top = -INFINITY; }
                     const float m_new = fmaxf(m_used, top * p.scale_log2);
                     const bool grow = m_new > m_used + RESCALE_STEP;      // also true for the first finite maximum
                     const float alpha = grow ? (m_used == -INFINITY ? 0.0f : fast_exp2(m_used - m_new)) : 1.0f;
