@@ -535,7 +535,7 @@ long long scratch_of(int requests, int beams, int vocab, int wanted) {
 MLB_EXPORT int mlb_beam_select(const void* logits, int dtype, long long ld, const float* scores, const int* ended, int end_token, int requests, int beams,
                                int vocab, int wanted, float* out_scores, int* out_parents, int* out_tokens, void* scratch, long long scratch_bytes,
                                cudaStream_t stream) {
-    if (requests < 0 || beams <= 0 || beams > MAX_BEAMS || vocab <= 0 || ld < vocab || wanted <= 0 || wanted > MAX_WANTED)
+    if (requests < 0 || beams <= 0 || beams > MAX_BEAMS || vocab <= 0 || vocab > (1 << 30) || ld < vocab || wanted <= 0 || wanted > MAX_WANTED)
         return fail(MLB_UNSUPPORTED_SIZE, "beam_select: %d requests of %d beams, vocabulary %d, %d wanted (at most %d beams, %d wanted)", requests, beams,
                     vocab, wanted, MAX_BEAMS, MAX_WANTED);
     if ((long long)beams * vocab >= (1ll << 31) || (long long)requests * beams > 65535)

@@ -178,7 +178,7 @@ struct AcceptParams {
     int* counts;             // [A]
     int* following;          // [A]
     int* error_flag;
-    int width, max_blocks, storages, write;
+    int nodes, width, max_blocks, storages, write;       // nodes: T
 };
 
 template <int VEC>
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(THREADS) accept_kernel(const __grid_constant__
     const int a = blockIdx.y, tid = threadIdx.x;
     const int start = p.starts[a];
     int n = p.starts[a + 1] - start;
-    if (n < 0 || n > MAX_NODES || n > p.width) {
+    if (n < 0 || n > MAX_NODES || n > p.width || start < 0 || start + n > p.nodes) {
         if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 3);
         n = 0;
     }
@@ -374,14 +374,14 @@ MLB_EXPORT int mlb_reorder_pages(const void* const* bases, int count, long long 
 }
 
 MLB_EXPORT int mlb_accept_drafts(const void* const* bases, int count, long long num_pages, int page_size, int planes, int row, int planes2, int row2,
-                                 const int* tokens, const int* parents, const int* choices, const int* starts, const int* lengths, int sequences,
+                                 const int* tokens, const int* parents, const int* choices, const int* starts, const int* lengths, int nodes, int sequences,
                                  const int* table, int max_blocks, int* path, int width, int* counts, int* following, int write, int* error_flag,
                                  cudaStream_t stream) {
     Storages s;
     int status = take_storages(s, bases, count, "accept_drafts");
     if (status != MLB_OK) return status;
     AcceptParams p{PageLayout{num_pages, page_size, planes, row, planes2, row2}, tokens, parents, choices, starts, lengths, table, path, counts,
-                   following, error_flag, width, max_blocks, count, write};
+                   following, error_flag, nodes, width, max_blocks, count, write};
     if (count && (status = check_layout(p.at, "accept_drafts")) != MLB_OK) return status;
     if (sequences < 0 || sequences > 65535 || width <= 0 || (count && max_blocks <= 0)) return fail(MLB_INVALID_ARGUMENT, "accept_drafts: bad sizes");
     if (sequences == 0) return MLB_OK;

@@ -25,7 +25,7 @@ constexpr int MAX_WORDS = MAX_NODES / 32;
 // ------------------------------------------------------------------------------ masks
 // A thread a node, walking up; a parent is an earlier node of the sequence or -1, so a walk ends.
 __global__ void __launch_bounds__(MAX_NODES) draft_masks_kernel(const int* __restrict__ parents, const int* __restrict__ starts, const int* __restrict__ lengths,
-                                                                int words, int* __restrict__ masks, int* __restrict__ positions, int* __restrict__ places,
+                                                                int tokens, int words, int* __restrict__ masks, int* __restrict__ positions, int* __restrict__ places,
                                                                 int* error_flag) {
     pdl_prologue();
     __shared__ int s_parent[MAX_NODES];
@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(MAX_NODES) draft_masks_kernel(const int* __res
     const int a = blockIdx.x, i = threadIdx.x;
     const int start = starts[a], length = lengths[a];
     int n = starts[a + 1] - start;
-    if (n < 0 || n > words * 32) {
+    if (n < 0 || n > words * 32 || start < 0 || start + n > tokens) {
         if (i == 0 && error_flag) atomicExch(error_flag, 3);
         n = 0;
     }
@@ -138,6 +138,10 @@ __global__ void __launch_bounds__(groups<T, DMAX>() * THREADS, 1) draft_attentio
     const int G = p.group, D = p.dim;
     const int rows = min(ROWS, n * G - row0);
     if (rows <= 0) return;
+    if (start < 0 || start + n > p.tokens) {                   // rows that are not there
+        if (threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 3);
+        return;
+    }
     if (n > p.max_nodes && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 3);      // the grid has no rows for the last of them
     // The shares begin at the first key that a row may see (positions are at least `length`); the last one takes what is left, so that a
     // sequence longer than the caller said costs time and nothing else.
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(THREADS) draft_join_kernel(DraftParams p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, seq = blockIdx.y;
     const int start = p.starts[seq], n = p.starts[seq + 1] - start;
     const int at = blockIdx.x * (THREADS / 32) + warp;
-    if (at >= n * p.heads) return;
+    if (at >= n * p.heads || start < 0 || start + n > p.tokens) return;
     const size_t row = (size_t)start * p.heads + at, all_rows = (size_t)p.tokens * p.heads;
     const int length = p.lengths[seq], keys = length + n - first_key(length, p.window) / KEYS * KEYS;
     const int shares = min(p.shares, (keys + p.share - 1) / p.share);
@@ -390,11 +394,11 @@ int run_attention(const DraftParams& p, int sequences, int max_nodes, cudaStream
 
 }  // namespace
 
-MLB_EXPORT int mlb_draft_masks(const int* parents, const int* starts, const int* lengths, int sequences, int words, int* masks, int* positions,
+MLB_EXPORT int mlb_draft_masks(const int* parents, const int* starts, const int* lengths, int tokens, int sequences, int words, int* masks, int* positions,
                                int* places, int* error_flag, cudaStream_t stream) {
     if (sequences < 0 || words <= 0 || words > MAX_WORDS) return fail(MLB_UNSUPPORTED_SIZE, "draft_masks: %d words a mask (at most %d)", words, MAX_WORDS);
     if (sequences == 0) return MLB_OK;
-    launch_kernel(draft_masks_kernel, sequences, words * 32, 0, stream, parents, starts, lengths, words, masks, positions, places, error_flag);
+    launch_kernel(draft_masks_kernel, sequences, words * 32, 0, stream, parents, starts, lengths, tokens, words, masks, positions, places, error_flag);
     return check_launch("draft_masks");
 }
 

@@ -279,7 +279,8 @@ struct Sequence {
 __device__ __forceinline__ Sequence sequence_at(const TcParams& p, int a) {
     Sequence s;
     s.token0 = p.starts[a];
-    s.n = min(p.starts[a + 1] - s.token0, p.max_nodes);
+    const int end = p.starts[a + 1];
+    s.n = s.token0 < 0 || end > p.tokens ? 0 : min(end - s.token0, p.max_nodes);      // (rows that are not there: the flag is raised where the kernel begins)
     s.length = p.lengths[a];
     s.lo = p.window > 0 ? max(0, s.length - p.window + 1) : 0;
     s.first = s.lo / BN;
@@ -463,7 +464,7 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         }
     } else if (warp == 4 && blockIdx.x == 0) {
         for (int a = lane; a < p.sequences; a += 32)
-            if (p.starts[a + 1] - p.starts[a] > p.max_nodes && p.error_flag) atomicExch(p.error_flag, 3);
+            if ((p.starts[a + 1] - p.starts[a] > p.max_nodes || p.starts[a] < 0 || p.starts[a + 1] > p.tokens) && p.error_flag) atomicExch(p.error_flag, 3);
     }
     tc_fence_before();
     __syncthreads();

@@ -24,7 +24,7 @@ _PAGES = [c_void_p, c_int, c_longlong, c_int, c_int, c_int, c_int, c_int]       
 ops.register_signatures("cache_moves.cu", {
     "mlb_reorder_slots": [c_void_p, c_int, c_longlong, c_longlong, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p],
     "mlb_reorder_pages": [*_PAGES, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p],
-    "mlb_accept_drafts": [*_PAGES, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
+    "mlb_accept_drafts": [*_PAGES, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
                           c_int, c_void_p, c_void_p],
 })
 

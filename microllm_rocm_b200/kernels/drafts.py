@@ -25,7 +25,7 @@ TC_HEAD_DIMS, TC_KEYS, TC_ROWS = (64, 128), 128, 128        # csrc/drafts_tc.cu:
 TC_STRETCH = 2              # units (row tile x key tile) a CTA takes at least: a turn of both streams
 
 ops.register_signatures("drafts.cu", {
-    "mlb_draft_masks": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "mlb_draft_masks": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "mlb_draft_attention": [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
                             c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
 })
@@ -82,7 +82,7 @@ def draft_masks(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tens
         need_on(device, (error_flag, "error_flag", INT, 1))
     need_current(device, "draft_masks")
     L = ops.lib("drafts.cu")
-    build.check(L, L.mlb_draft_masks(parents.data_ptr(), starts.data_ptr(), lengths.data_ptr(), sequences, masks.shape[1], masks.data_ptr(), positions.data_ptr(),
+    build.check(L, L.mlb_draft_masks(parents.data_ptr(), starts.data_ptr(), lengths.data_ptr(), T, sequences, masks.shape[1], masks.data_ptr(), positions.data_ptr(),
                                      _address(places), _address(error_flag), ops._stream()))
 
 
@@ -191,7 +191,7 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
         return
     need_current(device, "accept_drafts")
     L = ops.lib("cache_moves.cu")
-    trees = (tokens.data_ptr(), parents.data_ptr(), choices.data_ptr(), starts.data_ptr(), lengths.data_ptr(), sequences)
+    trees = (tokens.data_ptr(), parents.data_ptr(), choices.data_ptr(), starts.data_ptr(), lengths.data_ptr(), T[0], sequences)
     for i, (address, count, layout, _) in enumerate(groups or [(0, 0, (1, 1, 1, 1, 0, 0), None)]):
         build.check(L, L.mlb_accept_drafts(address, count, *layout, *trees, _address(block_table), block_table.shape[1] if block_table is not None else 0,
                                            path.data_ptr(), path.shape[1], counts.data_ptr(), following.data_ptr(), 1 if i == 0 else 0,

@@ -563,3 +563,37 @@ def test_attention_does_not_depend_on_which_warp_is_late(lag, monkeypatch):
     monkeypatch.setitem(ops.TEST_DEFINES, source, {k: v for k, v in defines.items() if k != "HEAD_DIM"})
     for s, w in zip(steps, want):
         assert torch.equal(s.run(), w) and int(s.error) == 0
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 32), (BF16, 128)])
+def test_starts_beyond_the_rows_raise_the_flag(dtype, dim):
+    """A list of starts that names rows that are not there: nothing is read or written for that sequence."""
+    step = Step(dtype, 6, 2, dim, 16, [40, 90], [[-1, 0, 0], [-1, 0, 1, 1]], 3)
+    want = step.want()
+    step.starts = [0, 3, 9]
+    got = step.run()
+    assert int(step.error) == 3 and (got[3:] == 7.0).all()
+    step.check(got[:3], want[:3], error=3)
+    masks, positions, error = dev_ints([[5]] * 7), dev_ints([5] * 7), dev_ints([0])
+    drafts.draft_masks(dev_ints([-1, 0, 0, -1, 0, 1, 1]), dev_ints([0, 3, 9]), dev_ints([40, 90]), masks, positions, None, error)
+    assert int(error) == 3 and masks[3:].tolist() == [[5]] * 4 and masks[:3].tolist() == [[1], [3], [5]]
+    path, counts, following, error = dev_ints([[7] * 6] * 2), dev_ints([7, 7]), dev_ints([7, 7]), dev_ints([0])
+    drafts.accept_drafts(dev_ints([1] * 7), dev_ints([-1, 0, 0, -1, 0, 1, 1]), dev_ints([1] * 7), dev_ints([0, 3, 9]), dev_ints([40, 90]), path, counts, following,
+                         error_flag=error)
+    assert int(error) == 3 and counts.tolist() == [2, 0] and path[1].tolist() == [-1] * 6
+
+
+def test_a_chain_of_the_most_nodes_and_the_widest_masks():
+    step = Step(BF16, 4, 2, 128, 16, [70, 3], [list(range(-1, 255)), [-1]], 5)
+    step.check(step.run())
+    step = Step(F32, 2, 1, 32, 16, [70], [[-1] + [0] * 255], 5, window=20)
+    step.check(step.run())
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 64), (BF16, 64)])
+def test_many_sequences_and_whole_items(dtype, dim):
+    """More sequences than a warp looks at in one go, most of them in one CTA as a whole."""
+    rng = random.Random(8)
+    sizes = [rng.choice((0, 1, 2, 7)) for _ in range(75)]
+    step = Step(dtype, 2, 1, dim, 16, [rng.randrange(0, 90) for _ in sizes], [random_tree(rng, n) if n else [] for n in sizes], 4)
+    step.check(step.run())
