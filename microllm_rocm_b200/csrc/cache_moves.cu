@@ -121,14 +121,20 @@ __global__ void __launch_bounds__(THREADS) reorder_pages_kernel(const __grid_con
         s_parent[tid] = parent == tid ? -1 : parent;
     }
     __syncthreads();
-    const int first = max(0, p.first[request]), tokens = p.last[request] - first;
+    const int first = max(0, p.first[request]);
+    long long last = p.last[request];
+    if (last > (long long)p.max_blocks * p.at.page_size) {                   // a block beyond the table
+        if (tid == 0 && p.error_flag) atomicExch(p.error_flag, 2);
+        last = (long long)p.max_blocks * p.at.page_size;
+    }
+    const int tokens = (int)max(last - first, 0ll);
     char* const base = s.base[blockIdx.y];
     const int* const table = p.table + (size_t)request * p.beams * p.max_blocks;
     const long long page_bytes = p.at.bytes();
     // Neighbouring threads take neighbouring pieces of a row, then neighbouring tokens, then the next plane: within a page that is the order
     // of memory.
     const int per = p.at.row / VEC, per2 = p.at.row2 / VEC;
-    const long long firsts = (long long)p.at.planes * per * max(tokens, 0), items = firsts + (long long)p.at.planes2 * per2 * max(tokens, 0);
+    const long long firsts = (long long)p.at.planes * per * tokens, items = firsts + (long long)p.at.planes2 * per2 * tokens;
     for (long long i = (long long)blockIdx.x * THREADS + tid; i < items; i += (long long)gridDim.x * THREADS) {
         const bool second = i >= firsts;
         const int each = second ? per2 : per, row = second ? p.at.row2 : p.at.row;
@@ -137,10 +143,6 @@ __global__ void __launch_bounds__(THREADS) reorder_pages_kernel(const __grid_con
         const int place = first + t, block = place / p.at.page_size;
         const long long inside = (second ? (long long)p.at.planes * p.at.page_size * p.at.row : 0) +
                                  ((long long)plane * p.at.page_size + place % p.at.page_size) * row + piece * VEC;
-        if (block >= p.max_blocks) {
-            if (p.error_flag) atomicExch(p.error_flag, 2);
-            continue;
-        }
         T v[B];
         int to[B];
 #pragma unroll
@@ -149,11 +151,11 @@ __global__ void __launch_bounds__(THREADS) reorder_pages_kernel(const __grid_con
             if (s_parent[b] < 0) continue;
             const int from = table[(size_t)s_parent[b] * p.max_blocks + block];
             to[b] = table[(size_t)b * p.max_blocks + block];
-            if (from >= p.at.num_pages || to[b] >= p.at.num_pages) {
+            if (from < 0) to[b] = -1;              // a block that a window gave back: nobody reads it any more
+            else if (from >= p.at.num_pages || to[b] >= p.at.num_pages || to[b] < 0) {
                 if (p.error_flag) atomicExch(p.error_flag, 2);
                 to[b] = -1;
             }
-            if (from < 0) to[b] = -1;              // a block that a window gave back: nobody reads it any more
             if (to[b] >= 0) v[b] = *reinterpret_cast<const T*>(base + from * page_bytes + inside);
         }
 #pragma unroll

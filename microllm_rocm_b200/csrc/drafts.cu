@@ -10,6 +10,8 @@
 //   draft_join_kernel         joins the shares of the keys where they were split
 //
 // The tensor-core kernel for bf16 heads of 64 and 128 is csrc/drafts_tc.cu.
+#include <algorithm>
+
 #include "common.cuh"
 #include "packed.cuh"
 
@@ -78,6 +80,7 @@ struct DraftParams {
     const int* table;        // [A, max_blocks]
     int words, max_blocks, num_pages, page_size;
     int heads, kv_heads, group, dim, window, row_tiles;
+    int reach;               // keys that a row of the table has blocks for
     int share;               // keys of one share, a multiple of KEYS
     int shares;
     int tokens, max_nodes;
@@ -142,6 +145,10 @@ __global__ void __launch_bounds__(groups<T, DMAX>() * THREADS, 1) draft_attentio
         if (threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 3);
         return;
     }
+    if (length < 0 || length > p.reach - n) {                  // keys that are not
+        if (threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 2);
+        return;
+    }
     if (n > p.max_nodes && threadIdx.x == 0 && p.error_flag) atomicExch(p.error_flag, 3);      // the grid has no rows for the last of them
     // The shares begin at the first key that a row may see (positions are at least `length`); the last one takes what is left, so that a
     // sequence longer than the caller said costs time and nothing else.
@@ -156,7 +163,7 @@ __global__ void __launch_bounds__(groups<T, DMAX>() * THREADS, 1) draft_attentio
     auto place_of = [&](int key) -> long long {
         if (key < lo || key >= key_end) return -1;
         const int block = key / p.page_size;
-        const int page = block < p.max_blocks ? table[block] : -1;
+        const int page = table[block];
         if (page < 0 || page >= p.num_pages) {
             if (p.error_flag) atomicExch(p.error_flag, 2);
             return -1;
@@ -249,7 +256,7 @@ __global__ void __launch_bounds__(groups<T, DMAX>() * THREADS, 1) draft_attentio
             if (key >= length) seen = seen && ((mask_s[r][min((key - length) >> 5, MAX_WORDS - 1)] >> ((key - length) & 31)) & 1u) && (key - length) < p.words * 32;
             const float x = seen ? s[i] * p.scale : -INFINITY;
             const float m_new = fmaxf(m[i], warp_max(x));
-            const float e = seen ? expf(x - m_new) : 0.0f;
+            const float e = x == -INFINITY ? 0.0f : expf(x - m_new);
             const float alpha = m[i] == -INFINITY ? 0.0f : expf(m[i] - m_new);
             l[i] = l[i] * alpha + warp_sum(e);
             m[i] = m_new;
@@ -334,6 +341,7 @@ __global__ void __launch_bounds__(THREADS) draft_join_kernel(DraftParams p) {
     if (at >= n * p.heads || start < 0 || start + n > p.tokens) return;
     const size_t row = (size_t)start * p.heads + at, all_rows = (size_t)p.tokens * p.heads;
     const int length = p.lengths[seq], keys = length + n - first_key(length, p.window) / KEYS * KEYS;
+    if (length < 0 || length > p.reach - n) return;
     const int shares = min(p.shares, (keys + p.share - 1) / p.share);
     const float2 mine = lane < shares ? p.part_norm[lane * all_rows + row] : make_float2(-INFINITY, 0.0f);       // of the first 32 shares
     float top = mine.x;
@@ -417,7 +425,7 @@ MLB_EXPORT int mlb_draft_attention(const void* q, const void* pages, void* out, 
     if (sequences > 65535 || row_tiles * kv_heads > 65535) return fail(MLB_UNSUPPORTED_SIZE, "draft_attention: too many sequences or rows");
     if (tokens == 0 || sequences == 0) return MLB_OK;
     DraftParams p{q, pages, out, starts, lengths, positions, masks, table, words, max_blocks, num_pages, page_size, heads, kv_heads, group, dim, window,
-                  row_tiles, share, shares, tokens, max_nodes, scale, nullptr, nullptr, error_flag};
+                  row_tiles, (int)std::min((long long)max_blocks * page_size, 1ll << 30), share, shares, tokens, max_nodes, scale, nullptr, nullptr, error_flag};
     p.part_norm = (float2*)scratch;
     p.part_out = (float*)scratch + (size_t)2 * shares * tokens * heads;
     if (dtype == MLB_F32) return run_attention<float>(p, sequences, max_nodes, stream);

@@ -28,6 +28,8 @@
 
 #include <cuda.h>
 
+#include <algorithm>
+
 #ifndef HEAD_DIM
 #error "compile with -DHEAD_DIM=64 or 128"
 #endif
@@ -47,7 +49,7 @@ constexpr int ROW_BYTES = 128;               // one swizzle span
 constexpr int Q_BYTES = SPANS * BM * ROW_BYTES;
 constexpr int KV_BYTES = SPANS * BN * ROW_BYTES;
 constexpr int SLOTS = D == 128 ? 5 : 8;
-constexpr int SHARED_BYTES = 3072;           // barriers and what the warps tell one another, behind the tiles
+constexpr int SHARED_BYTES = 3 << 10;          // barriers and what the warps tell one another, behind the tiles
 constexpr int SMEM_BYTES = 2 * Q_BYTES + SLOTS * KV_BYTES + SHARED_BYTES;
 static_assert(SMEM_BYTES <= 227 * 1024, "a CTA's shared memory");
 constexpr int THREADS = 384;
@@ -75,6 +77,7 @@ struct TcParams {
     int heads, kv_heads, group, tile_nodes, row_tiles, window, max_nodes;      // row_tiles: of a sequence of max_nodes
     int stretch;                    // units of a CTA at least
     int ctas, sequences, tokens;
+    int reach;                      // keys that a row of the table has blocks for
     float scale_log2;
     float* part_out;                // [ctas, 2, 2, D, BM]: of the item that a CTA's stretch begins in, and of the one that it ends in; a column's rows together
     float2* part_norm;              // [ctas, 2, 2, BM]
@@ -257,7 +260,6 @@ __device__ __forceinline__ float row_exp2(uint32_t (&s)[N], float scale, float s
     return (low(chains[0]) + high(chains[0])) + (low(chains[1]) + high(chains[1]));
 }
 
-
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
@@ -282,6 +284,7 @@ __device__ __forceinline__ Sequence sequence_at(const TcParams& p, int a) {
     const int end = p.starts[a + 1];
     s.n = s.token0 < 0 || end > p.tokens ? 0 : min(end - s.token0, p.max_nodes);      // (rows that are not there: the flag is raised where the kernel begins)
     s.length = p.lengths[a];
+    if (s.length < 0 || s.length > p.reach - s.n) s.length = s.n = 0;                 // (so are keys that are not)
     s.lo = p.window > 0 ? max(0, s.length - p.window + 1) : 0;
     s.first = s.lo / BN;
     s.tiles = s.n > 0 ? (s.length + s.n + BN - 1) / BN - s.first : 0;
@@ -463,8 +466,14 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             sh.lead = cut.lead;
         }
     } else if (warp == 4 && blockIdx.x == 0) {
-        for (int a = lane; a < p.sequences; a += 32)
-            if ((p.starts[a + 1] - p.starts[a] > p.max_nodes || p.starts[a] < 0 || p.starts[a + 1] > p.tokens) && p.error_flag) atomicExch(p.error_flag, 3);
+        for (int a = lane; a < p.sequences; a += 32) {
+            const int start = p.starts[a], end = p.starts[a + 1], length = p.lengths[a];
+            if (start < 0 || end > p.tokens || end - start > p.max_nodes) {
+                if (p.error_flag) atomicExch(p.error_flag, 3);
+            } else if (end > start && (length < 0 || length > p.reach - (end - start))) {
+                if (p.error_flag) atomicExch(p.error_flag, 2);
+            }
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -986,7 +995,6 @@ EncodeTiledFn encode_fn() {
     return fn;
 }
 
-
 int encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return fail(MLB_CUDA_ERROR, "draft_attention_tc: cuTensorMapEncodeTiled is not available from this driver");
@@ -1039,7 +1047,8 @@ MLB_EXPORT int mlb_draft_attention_tc(const void* q, const void* pages, void* ou
         if (status != MLB_OK) return status;
     }
     TcParams p{(__nv_bfloat16*)out, starts, lengths, positions, masks, table, words, max_blocks, num_pages, page_size, BN / page_size, heads, kv_heads, group,
-               tile_nodes, (max_nodes + tile_nodes - 1) / tile_nodes, window, max_nodes, stretch, ctas, sequences, tokens, scale * LOG2E, nullptr, nullptr, nullptr, error_flag};
+               tile_nodes, (max_nodes + tile_nodes - 1) / tile_nodes, window, max_nodes, stretch, ctas, sequences, tokens,
+               (int)std::min((long long)max_blocks * page_size, 1ll << 30), scale * LOG2E, nullptr, nullptr, nullptr, error_flag};
     if (ctas > 1) {
         p.part_out = (float*)scratch;
         p.part_norm = (float2*)(p.part_out + (size_t)ctas * 4 * BM * D);

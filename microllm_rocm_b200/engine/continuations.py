@@ -159,13 +159,17 @@ def beam_search(engine: Engine, prompt: Sequence[int], num_beams: int, max_new_t
 def _search(engine, names, prompt, max_new_tokens, end_token, device, vocab):
     cache, B = engine.cache, len(names)
     slots = ops.upload([[cache.slot(n) for n in names]], "int32", device)
+    portion = engine.max_step_tokens or len(prompt)
 
     def follow(parents: torch.Tensor, first: int, last: int, lagging) -> None:
         """Beams take their parents' tokens [first, last) and state; `lagging`: the beams whose books do not say `last` yet."""
         for name in lagging:
-            if not cache.reserve(name, last):
-                raise OutOfPages(f"no pages left for a beam to hold {last} tokens")
-            cache.commit(name, last)
+            # (a portion at a time, as its parent's came: a window's pool holds no more)
+            for at in range(cache.length(name), last, portion):
+                to = min(at + portion, last)
+                if not cache.reserve(name, to):
+                    raise OutOfPages(f"no pages left for a beam to hold {to} tokens")
+                cache.commit(name, to)
         if last > first:
             bounds = ops.upload([first, last], "int32", device)
             for group in cache.groups:
@@ -173,7 +177,6 @@ def _search(engine, names, prompt, max_new_tokens, end_token, device, vocab):
                 cache_moves.reorder_pages(cache.page_moves(group), table, parents, bounds[:1], bounds[1:], last - first, engine.error_flag)
         cache_moves.reorder_slots(cache.slot_moves(), slots, parents, engine.error_flag)
 
-    portion = engine.max_step_tokens or len(prompt)
     for at in range(0, len(prompt), portion):
         some = prompt[at:at + portion]
         logits = engine.step([StepEntry(names[0], some, [len(some) - 1] if at + portion >= len(prompt) else [])])

@@ -148,8 +148,8 @@ def reorder_pages(moves: PageMoves, block_table: torch.Tensor, parents: torch.Te
                   error_flag: Optional[torch.Tensor] = None) -> None:
     """In every pool: tokens first[r] .. last[r] - 1 of beam b (row r * beams + b of `block_table`) <- what its parent's pages held at these places
     before the call.  `parents` [requests, beams], `first` and `last` [requests], `block_table` [requests * beams, blocks], all int32.
-    Beams have pages of their own for these tokens.  Blocks that a window gave back (negative entries) are skipped; an
-    entry beyond the pool, a block beyond the table or a parent out of range raises the error flag and is skipped.
+    Beams have pages of their own for these tokens.  Blocks of the parent that a window gave back (negative entries) are skipped; an entry
+    beyond the pool, a beam without a page where its parent has one, a block beyond the table or a parent out of range raises the error flag and is skipped.
     `max_tokens`: the most tokens of a request (what the launch is sized for; more are moved all the same)."""
     if not isinstance(moves, PageMoves):
         raise KernelError("reorder_pages moves the storages of a PageMoves")

@@ -21,6 +21,7 @@ from .device import sm_count
 MAX_NODES = 256             # csrc/drafts.cu: nodes of a sequence
 ROWS, KEYS = 16, 32         # csrc/drafts.cu: rows (node, head of a group) and keys a CTA works on at a time
 SHARE_KEYS = 128            # keys below which a share is not cut further: a tile for each group of a CTA
+MAX_WINDOW = 1 << 30        # keys of a sequence at most
 TC_HEAD_DIMS, TC_KEYS, TC_ROWS = (64, 128), 128, 128        # csrc/drafts_tc.cu: keys a tile, rows of a stream (a CTA has two)
 TC_STRETCH = 2              # units (row tile x key tile) a CTA takes at least: a turn of both streams
 
@@ -112,7 +113,8 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     `q` and `out` [T, heads * D], `pages` [pages, 2, kv heads, page, D] of the same type (fp32 or bf16); `positions` and `masks` as `draft_masks`
     makes them (any other mask over a sequence's nodes will do); `block_table` [sequences, blocks] int32.
     `max_nodes`: the most nodes of a sequence, which the launch is sized for (a sequence of more raises the error flag).  `max_length`: the most keys
-    of a sequence, its nodes among them (how the work is cut; a longer sequence costs time only).  `alloc(bytes)` -> uint8 tensor: the step's own memory
+    of a sequence, its nodes among them (how the work is cut; a longer sequence costs time only).  A sequence that its row of `block_table` has no blocks for,
+    or whose `starts` name rows that are not there, raises the flag and is left out; a page that is not there raises it.  `alloc(bytes)` -> uint8 tensor: the step's own memory
     for partial results, for a caller whose launches are recorded and issued again; else it is taken and given back in the current stream's order."""
     device = q.get_device()
     tag, dtype = ops.dtype_tag(q), q.dtype
@@ -131,6 +133,7 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
         raise KernelError(f"draft_attention: {max_nodes} nodes among {max_length} keys in masks of {words} words (at most {MAX_NODES // 32})")
     if window is not None and window <= 0:
         raise KernelError("draft_attention: a window has at least one key")
+    window = min(int(window), MAX_WINDOW) if window is not None else 0
     if error_flag is not None:
         need_on(device, (error_flag, "error_flag", INT, 1))
     if T == 0 or sequences == 0:
@@ -145,7 +148,7 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
         L = ops.lib("drafts_tc.cu", _TC_DEFINES[head_dim])
         build.check(L, L.mlb_draft_attention_tc(q_at, pages_at, out_at, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
                                                 masks.data_ptr(), words, block_table.data_ptr(), max_blocks, num_pages, page_size, T, sequences,
-                                                int(max_nodes), num_heads, num_kv_heads, float(scale), int(window or 0), TC_STRETCH, ctas, _address(scratch),
+                                                int(max_nodes), num_heads, num_kv_heads, float(scale), window, TC_STRETCH, ctas, _address(scratch),
                                                 _address(error_flag), ops._stream()))
         return
     keys = min(max_length, window + max_nodes + KEYS) if window else max_length
@@ -155,7 +158,7 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
     L = ops.lib("drafts.cu")
     build.check(L, L.mlb_draft_attention(q_at, pages_at, out_at, tag, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
                                          masks.data_ptr(), words, block_table.data_ptr(), max_blocks, num_pages, page_size, T, sequences, int(max_nodes),
-                                         num_heads, num_kv_heads, head_dim, float(scale), int(window or 0), share, shares, _address(scratch),
+                                         num_heads, num_kv_heads, head_dim, float(scale), window, share, shares, _address(scratch),
                                          _address(error_flag), ops._stream()))
 
 

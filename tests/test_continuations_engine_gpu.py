@@ -204,3 +204,18 @@ def test_beam_search_refuses_and_gives_everything_back(folders):
     assert llm.engine.cache.stats()["live_requests"] == 0
     got = llm.beam_search([1, 2, 3], 2, 5)
     assert len(got) == 2 and all(len(t) == 5 and math.isfinite(s) for t, s in got)
+
+
+def test_beam_search_in_windows_that_the_prompt_does_not_fit(folders):
+    """Windowed layers' pools are sized for a window and a portion of the prompt, and a prompt of many such portions goes through them beam by beam."""
+    config = tiny_config("b")
+    prompt = random_tokens(250, config.vocab_size, 6)
+    whole = LLM(folders["b"], dtype="float32", page_size=8, max_tokens=4096).beam_search(prompt, 4, 6)
+    engine = load_engine(folders["b"], dtype="float32", page_size=8, max_tokens=4 * 264, max_requests=4, max_step_tokens=16)
+    windowed = [g for g in engine.cache.groups.values() if g.window is not None]
+    assert windowed and all(g.pool.num_pages < 4 * 32 for g in windowed)          # fewer than four prompts take
+    from microllm_rocm_b200.engine.continuations import beam_search
+    got = beam_search(engine, prompt, 4, 6)
+    assert [t for t, _ in got] == [t for t, _ in whole]
+    assert all(abs(a - b) <= 6 * 4 * FP32_ATOL for (_, a), (_, b) in zip(got, whole))
+    engine.cache.check()

@@ -597,3 +597,56 @@ def test_many_sequences_and_whole_items(dtype, dim):
     sizes = [rng.choice((0, 1, 2, 7)) for _ in range(75)]
     step = Step(dtype, 2, 1, dim, 16, [rng.randrange(0, 90) for _ in sizes], [random_tree(rng, n) if n else [] for n in sizes], 4)
     step.check(step.run())
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 32), (BF16, 128)])
+@pytest.mark.parametrize("wrong", [-1, -500, 2 ** 31 - 1, 2000])
+def test_lengths_that_no_table_row_holds_raise_the_flag(dtype, dim, wrong):
+    """The sequence is left out; the others are as they were."""
+    step = Step(dtype, 6, 2, dim, 16, [40, 90, 7], [[-1, 0, 0], [-1, 0, 1, 1], [-1]], 3)
+    want = step.want()
+    step.lengths = [40, wrong, 7]
+    got = step.run()
+    assert int(step.error) == 2 and (got[3:7] == 7.0).all()
+    rest = [0, 1, 2, 7]
+    step.check(got[rest], want[rest], error=2)
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 32), (BF16, 128)])
+def test_scores_of_minus_infinity_weigh_nothing(dtype, dim):
+    """Two whole tiles of keys that every row scores -inf, in front of and among finite ones; and a sequence that has no others: zeros."""
+    step = Step(dtype, 4, 2, dim, 16, [600, 40], [[-1, 0, 0], [-1, 0]], 4)
+    step.q = step.q.abs()
+    clean = step.pages.clone()
+    for a, places in ((0, [*range(256), 300, 555]), (1, range(42))):
+        for j in places:
+            step.pages[step.table[a][j // 16], 0, :, j % 16, 1] = -math.inf
+    want = step.want()
+    assert torch.isnan(want[3:]).all() and torch.isfinite(want[:3]).all()
+    got = step.run()
+    step.pages = clean                             # (the bound goes by the sizes of the finite keys)
+    step.check(got[:3], want[:3])
+    assert (got[3:] == 0.0).all()
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 32), (BF16, 128)])
+def test_a_window_wider_than_any_sequence_is_none(dtype, dim):
+    step = Step(dtype, 4, 2, dim, 16, [200], [[-1, 0, 0, 2]], 4)
+    first = step.run()
+    for window in (204, 2 ** 31, 2 ** 40):
+        step.window = window
+        assert torch.equal(step.run(), first)
+
+
+def test_pages_want_a_page_wherever_the_parent_has_one():
+    pool = torch.randn(6, 4, 8, device=DEV)
+    kept = pool.clone()
+    error = dev_ints([0])
+    moves = cache_moves.PageMoves([pool], 4)
+    cache_moves.reorder_pages(moves, dev_ints([[2, 0], [-1, 1]]), dev_ints([[0, 0]]), dev_ints([0]), dev_ints([6]), 6, error)
+    kept[1, :2] = kept[0, :2]                      # the block that both have moves all the same
+    assert int(error) == 2 and torch.equal(pool, kept)
+    error.zero_()
+    cache_moves.reorder_pages(moves, dev_ints([[2, 0], [3, 1]]), dev_ints([[0, 0]]), dev_ints([0]), dev_ints([2 ** 31 - 1]), 8, error)
+    kept[3], kept[1] = kept[2], kept[0]            # as far as the table goes
+    assert int(error) == 2 and torch.equal(pool, kept)
