@@ -295,10 +295,12 @@ __device__ __forceinline__ Sequence sequence_at(const TcParams& p, int a) {
 // How the line is cut, by one whole warp: units a CTA, and for this CTA its stretch, the sequence that it begins in and that one's first unit.  CTA 0
 // leaves all sequences' first units for the join.
 //
-// Every item begins with `lead` units that stand for no work: what it costs a CTA to end one item (results out, accumulators free) and begin another is about
-// four turns' time, and without them the CTAs that hold an item's end and the next one's beginning were the last by a fifth of the kernel's time.  Short
-// stretches, where a call waits for the first tile and not for the last CTA, take less.
-constexpr int MOST_LEAD = 6;
+// Every item begins with `lead` units that stand for no work: what it costs a CTA to end one item (results out, accumulators free) and begin another.  CTAs' times in
+// eight calls of all kinds are 1.2 us a unit, 4.5 us an item, 1 us more a tile that needs masks, within 1 us; without `lead` the CTAs that hold an item's end and the
+// next one's beginning were the last by a fifth of the kernel's time.  4, 5 and 6 units at most: 16 sequences of up to 2,048 keys and 64 nodes 37.8, 37.5, 37.3 us a
+// layer, 4 of 8,192 keys 69.8, 70.1, 71.0.  Shorter stretches take less, and the shortest none (a unit more a CTA would be a turn more: one sequence of 2,074 keys and
+// 26 nodes, 12 heads of 2, 15.7 us instead of 17.3).
+constexpr int MOST_LEAD = 5;
 struct Cut {
     int stretch, lead, unit, end, a, base;
 };
@@ -318,7 +320,8 @@ __device__ __forceinline__ Cut cut_line(const TcParams& p, int lane) {
     total = __reduce_add_sync(0xffffffffu, total);
     items = __reduce_add_sync(0xffffffffu, items);
     Cut c;
-    c.lead = min(MOST_LEAD, (total + p.ctas - 1) / p.ctas / 2);
+    const int each = (total + p.ctas - 1) / p.ctas;
+    c.lead = each <= p.stretch ? 0 : min(MOST_LEAD, each);
     total += items * c.lead;
     c.stretch = max(p.stretch, (total + p.ctas - 1) / p.ctas);
     c.unit = min((int)blockIdx.x * c.stretch, total);
@@ -780,7 +783,7 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                             for (int i = 0; i < SPANS * 8; ++i) {
                                 uint32_t v[4];
                                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                                             : "r"(vrow + (i / 8) * (BN * ROW_BYTES) + (i % 8) * 16));
+                                             : "r"(vrow + (i / 8) * (BN * ROW_BYTES) + ((i ^ lane) & 7) * 16));      // neighbouring rows in different banks
 #pragma unroll
                                 for (int k = 0; k < 4; ++k) worst = __vmaxu2(worst, v[k] & 0x7f807f80u);
                             }
@@ -791,7 +794,7 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                         if (odd || nobodys) {
 #pragma unroll 1
                             for (int i = 0; i < SPANS * 8; ++i)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vrow + (i / 8) * (BN * ROW_BYTES) + (i % 8) * 16), "r"(0u) : "memory");
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vrow + (i / 8) * (BN * ROW_BYTES) + ((i ^ lane) & 7) * 16), "r"(0u) : "memory");
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // for the tensor core
                     }
