@@ -214,7 +214,9 @@ __device__ __forceinline__ bool is_far(float top) { return fabsf(top) > 1e37f; }
 // itself, so its rounding cancels).  A thread's pieces of the next slice come into its own places in shared memory while this one is worked on; nobody
 // else reads them, so nobody waits for anybody.
 //
-// What bounds it: with few rows a slice a CTA, and the way from the launch to the ranked list; with many rows the reading: TODO
+// What bounds it: with few rows a slice a CTA, and the way from the launch to the ranked list (8 rows of 151,936: 13 us with the join).  With many rows no one thing: 160
+// rows of 152,064 fp32 logits, a fifth of them not read (78 MB), take 30 us with the join, of which reading alone is 15, the join 6, the bound 2.6, the list 2.6, its
+// ranking 2.3 and the exponentials 1.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) select_slices_kernel(SelectParams p) {
     pdl_prologue();
@@ -374,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, 4) select_slices_kernel(SelectParams 
 }
 
 // What the parts left: up to AHEAD elements a thread are asked for at once, before the sums are joined (a call of few beams has that many; of more, the
-// rest is read when it is looked at).
+// rest is read when it is looked at).  A chain of round trips to memory and shared memory and no bandwidth: 6 us for 32 requests of 5 beams.
 constexpr int AHEAD = 12;
 __global__ void __launch_bounds__(THREADS) select_join_kernel(SelectParams p) {
     pdl_prologue();

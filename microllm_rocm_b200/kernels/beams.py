@@ -59,7 +59,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, out_scores: torch.Te
     need_current(device, "beam_select")
     L = ops.lib("beams.cu")
     nbytes = _scratch_bytes(rows, vocab, wanted)
-    scratch = ops.scratch(nbytes, logits.device, "beam_select")
+    scratch = ops.scratch(nbytes, logits, "beam_select")
     build.check(L, L.mlb_beam_select(logits.data_ptr(), tag, logits.stride(0) if rows > 1 else vocab, scores.data_ptr(), _address(ended), int(end_token) if ended is not None else -1,
                                      requests, beams, vocab, wanted, out_scores.data_ptr(), out_parents.data_ptr(), out_tokens.data_ptr(),
                                      scratch.data_ptr(), nbytes, ops._stream()))

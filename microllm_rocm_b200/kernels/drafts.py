@@ -20,10 +20,10 @@ from .device import sm_count
 
 MAX_NODES = 256             # csrc/drafts.cu: nodes of a sequence
 ROWS, KEYS = 16, 32         # csrc/drafts.cu: rows (node, head of a group) and keys a CTA works on at a time
-SHARE_KEYS = 128            # keys below which a share is not cut further: a tile for each group of a CTA
+SHARE_KEYS = 128            # a share is whole rounds of a CTA's groups, a tile of keys each (one of 724 keys: in shares of 128 18.8 us, of 256 25.9)
 MAX_WINDOW = 1 << 30        # keys of a sequence at most
 TC_HEAD_DIMS, TC_KEYS, TC_ROWS = (64, 128), 128, 128        # csrc/drafts_tc.cu: keys a tile, rows of a stream (a CTA has two)
-TC_STRETCH = 2              # units (row tile x key tile) a CTA takes at least: a turn of both streams
+TC_STRETCH = 2              # units (row tile x key tile) a CTA takes at least: a turn of both streams (one sequence of 2,074 keys 14.8 us a layer; 1: 16.3, 4: 19.7)
 
 ops.register_signatures("drafts.cu", {
     "mlb_draft_masks": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
@@ -88,9 +88,11 @@ def draft_masks(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tens
 
 
 def _shares(ctas: int, keys: int, sms: int):
-    """(keys a share, shares): the keys are split until two CTAs a multiprocessor have work, down to SHARE_KEYS."""
-    shares = max(1, min(-(-keys // SHARE_KEYS), 2 * sms // max(1, ctas)))
-    share = -(-(-(-keys // shares)) // KEYS) * KEYS
+    """(keys a share, shares): the keys are split until two CTAs a multiprocessor have work, down to a round of a CTA's groups, or four, down to four rounds;
+    always whole rounds.  (us a layer: 4 sequences of 500 to 2,000 keys, 6 heads of 32, 12 shares of 168 keys 22.4, 8 of 256 15.0; 4 of 1,000, 24 nodes, 12 heads of 128, 8
+    shares of 128 keys 59.4, 4 of 256 49.9; 16 of up to 2,000, 1 share 177, 2 of 1,024 160.)"""
+    shares = max(1, min(-(-keys // SHARE_KEYS), 2 * sms // max(1, ctas)), min(-(-keys // (4 * SHARE_KEYS)), 4 * sms // max(1, ctas)))
+    share = -(-(-(-keys // shares)) // SHARE_KEYS) * SHARE_KEYS
     return share, -(-keys // share)
 
 
@@ -100,7 +102,7 @@ def _ctas(heads: int, row_tiles: int, key_tiles: int, sms: int) -> int:
 
 
 def _memory(alloc, q: torch.Tensor, nbytes: int) -> torch.Tensor:
-    return ops.scratch(nbytes, q.device, "draft_attention") if alloc is None else alloc(nbytes)
+    return ops.scratch(nbytes, q, "draft_attention") if alloc is None else alloc(nbytes)
 
 
 def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor,

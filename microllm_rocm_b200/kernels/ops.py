@@ -744,11 +744,11 @@ def second_stream():
     return getattr(_launch_on, "side", None), getattr(_launch_on, "scratch", None)
 
 
-def scratch(nbytes: int, device: torch.device, what: str) -> torch.Tensor:
-    """Memory for one call's own use between its launches: the tensor framework's, which takes it back in the order of the current stream.  A
-    launch on the second stream is not in that order, so there it is the step's (`on_side_stream(scratch)`)."""
+def scratch(nbytes: int, like: torch.Tensor, what: str) -> torch.Tensor:
+    """Memory on `like`'s device for one call's own use between its launches: the tensor framework's, which takes it back in the order of the current
+    stream.  A launch on the second stream is not in that order, so there it is the step's (`on_side_stream(scratch)`)."""
     if _launch_on.__dict__.get("side") is None:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return like.new_empty(-(-nbytes // like.element_size()))      # (torch.empty takes half as long again)
     step_scratch = getattr(_launch_on, "scratch", None)
     if step_scratch is None:
         raise KernelError(f"{what}: on the second stream it needs the step's scratch memory (on_side_stream(scratch))")

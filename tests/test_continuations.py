@@ -147,10 +147,10 @@ def test_tensor_core_attention_takes_a_cta_a_multiprocessor_at_most():
 def test_scratch_on_the_second_stream_is_the_steps(monkeypatch):
     monkeypatch.setattr(ops._launch_on, "side", 7, raising=False)
     with pytest.raises(KernelError, match="second stream"):
-        ops.scratch(64, torch.device("cpu"), "beam_select")
+        ops.scratch(64, torch.empty(1), "beam_select")
     kept = torch.empty(64, dtype=torch.uint8)
     monkeypatch.setattr(ops._launch_on, "scratch", lambda n: kept[:n], raising=False)
-    assert ops.scratch(32, torch.device("cpu"), "beam_select").data_ptr() == kept.data_ptr()
+    assert ops.scratch(32, torch.empty(1), "beam_select").data_ptr() == kept.data_ptr()
 
 
 def test_error_texts():
