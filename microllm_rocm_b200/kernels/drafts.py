@@ -88,10 +88,13 @@ def draft_masks(parents: torch.Tensor, starts: torch.Tensor, lengths: torch.Tens
 
 
 def _shares(ctas: int, keys: int, sms: int):
-    """(keys a share, shares): the keys are split until two CTAs a multiprocessor have work, down to a round of a CTA's groups, or four, down to four rounds;
-    always whole rounds.  (us a layer: 4 sequences of 500 to 2,000 keys, 6 heads of 32, 12 shares of 168 keys 22.4, 8 of 256 15.0; 4 of 1,000, 24 nodes, 12 heads of 128, 8
-    shares of 128 keys 59.4, 4 of 256 49.9; 16 of up to 2,000, 1 share 177, 2 of 1,024 160.)"""
-    shares = max(1, min(-(-keys // SHARE_KEYS), 2 * sms // max(1, ctas)), min(-(-keys // (4 * SHARE_KEYS)), 4 * sms // max(1, ctas)))
+    """(keys a share, shares): the keys are split until two CTAs a multiprocessor have work, down to a round of a CTA's groups, always into whole rounds; where there are
+    more CTAs than multiprocessors already, until there are four, down to four rounds.  (us a layer: 4 sequences of 500 to 2,000 keys, 6 heads of 32, 12 shares of 168 keys
+    22.4, 8 of 256 15.0; 4 of 1,000, 24 nodes, 12 heads of 128, 8 shares of 128 keys 59.4, 4 of 256 49.9; 16 of up to 2,000, 1 share 177, 2 of 1,024 160.)"""
+    most, least = 2 * sms // max(1, ctas), SHARE_KEYS
+    if ctas > sms:
+        most, least = 4 * sms // ctas, 4 * SHARE_KEYS
+    shares = max(1, min(-(-keys // least), most))
     share = -(-(-(-keys // shares)) // SHARE_KEYS) * SHARE_KEYS
     return share, -(-keys // share)
 

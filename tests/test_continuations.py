@@ -133,11 +133,11 @@ def test_storages_of_one_layout_share_a_launch():
                                                                         (1, (5, 8, 2, 12, 2, 16))]
 
 
-@pytest.mark.parametrize("ctas, keys", [(1, 1), (1, 63), (1, 64), (1, 5000), (3, 131072), (148, 1000), (297, 64), (5000, 100000)])
+@pytest.mark.parametrize("ctas, keys", [(1, 1), (1, 63), (1, 64), (1, 5000), (3, 131072), (148, 1000), (200, 5000), (297, 64), (5000, 100000)])
 def test_shares_cover_the_keys(ctas, keys):
     share, shares = drafts._shares(ctas, keys, 148)
-    assert share % drafts.KEYS == 0 and shares >= 1 and share * shares >= keys and share * (shares - 1) < keys
-    assert ctas * shares <= max(2 * 148, ctas)
+    assert share % drafts.SHARE_KEYS == 0 and shares >= 1 and share * shares >= keys and share * (shares - 1) < keys
+    assert ctas * shares <= max((4 if ctas > 148 else 2) * 148, ctas)
 
 
 def test_tensor_core_attention_takes_a_cta_a_multiprocessor_at_most():
