@@ -37,6 +37,7 @@ class DraftStep:
     entries: List[DraftEntry]
     logits: torch.Tensor
     ctx: object
+    held: List[object]            # the requests' books
 
 
 @dataclass
@@ -95,15 +96,15 @@ def draft_step(engine: Engine, entries: Sequence[DraftEntry]) -> DraftStep:
     logits = engine.model.forward(ctx, engine.cache_views(ctx))
     engine.steps_run += 1
     engine.tokens_run += T
-    return DraftStep(entries, logits, ctx)
+    return DraftStep(entries, logits, ctx, [engine.cache.requests[e.request] for e in entries])
 
 
 def accept_drafts(engine: Engine, step: DraftStep, choices: torch.Tensor) -> List[Accepted]:
     """Walk each tree of `step` along `choices` ([nodes] int32 on the device: the model's own token behind every node), keep the branch in the
     cache and commit it.  Nothing else may have run for these requests since the step."""
     ctx, cache = step.ctx, engine.cache
-    for e, n in zip(step.entries, ctx.seq_pos0_host):
-        if not cache.has(e.request) or cache.length(e.request) != n:
+    for e, n, held in zip(step.entries, ctx.seq_pos0_host, step.held):
+        if cache.requests.get(e.request) is not held or cache.length(e.request) != n:
             raise StepError(f"request {e.request!r} went on since its draft step")
     A, most = ctx.num_seqs, ctx.tree[2]
     result = torch.empty(A * (most + 2), dtype=torch.int32, device=engine.device)

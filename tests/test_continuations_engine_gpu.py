@@ -219,3 +219,39 @@ def test_beam_search_in_windows_that_the_prompt_does_not_fit(folders):
     assert [t for t, _ in got] == [t for t, _ in whole]
     assert all(abs(a - b) <= 6 * 4 * FP32_ATOL for (_, a), (_, b) in zip(got, whole))
     engine.cache.check()
+
+
+def test_a_request_that_was_released_and_added_again_is_another_one(folders):
+    engine = load_engine(folders["a"], dtype="float32", page_size=8, max_tokens=64)
+    assert engine.cache.add("r")
+    engine.step([StepEntry("r", [1, 2, 3])])
+    step = engine.draft_step([DraftEntry("r", [4, 5], [-1, 0])])
+    engine.cache.release("r")
+    assert engine.cache.add("r")
+    engine.step([StepEntry("r", [6, 7, 8])])
+    with pytest.raises(StepError, match="went on"):
+        engine.accept_drafts(step, argmax(step.logits))
+    with pytest.raises(StepError):
+        engine.draft_step([])
+    with pytest.raises(StepError, match="no tokens"):
+        engine.draft_step([DraftEntry("r", [], [])])
+
+
+@pytest.mark.parametrize("steps", [1, 2, 4, 7])
+def test_a_search_beside_requests_that_the_scheduler_holds(folders, steps):
+    config = GenerationConfig(max_new_tokens=12, temperature=0.0)
+    prompts = [random_tokens(n, 384, n) for n in (5, 40, 17)]
+    alone = LLM(folders["b"], dtype="float32", page_size=8, max_tokens=2048)
+    want = alone.generate(prompts, config)
+    found = alone.beam_search(prompts[1], 3, 5)
+    llm = LLM(folders["b"], dtype="float32", page_size=8, max_tokens=2048)
+    names = [llm.submit(p, config) for p in prompts]
+    for _ in range(steps):
+        llm.step()
+    got = llm.beam_search(prompts[1], 3, 5)
+    assert [t for t, _ in got] == [t for t, _ in found]
+    assert all(abs(a - b) <= 5 * 4 * FP32_ATOL for (_, a), (_, b) in zip(got, found))
+    while llm.has_work():
+        llm.step()
+    llm.engine.cache.check()
+    assert [list(llm.poll(name).generated) for name in names] == want

@@ -650,3 +650,38 @@ def test_pages_want_a_page_wherever_the_parent_has_one():
     cache_moves.reorder_pages(moves, dev_ints([[2, 0], [3, 1]]), dev_ints([[0, 0]]), dev_ints([0]), dev_ints([2 ** 31 - 1]), 8, error)
     kept[3], kept[1] = kept[2], kept[0]            # as far as the table goes
     assert int(error) == 2 and torch.equal(pool, kept)
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 128), (BF16, 128), (BF16, 64)])
+def test_pages_beyond_32_bits(dtype, dim):
+    """A pool of more than 2^31 elements (and 2^32 bytes): what its last pages hold is read and moved as if they were the first."""
+    rng = random.Random(9)
+    step = Step(dtype, 4, 2, dim, 16, [300, 40], [random_tree(rng, 9), random_tree(rng, 5)], 7)
+    want = step.run()
+    step.check(want)
+    near = step.pages.to(DEV)
+    each = near[0].numel()
+    far = torch.empty((2 ** 31 // each + 1 + len(near), *near.shape[1:]), dtype=dtype, device=DEV)
+    shift = len(far) - len(near)
+    far[shift:] = near
+    tables = [dev_ints([[page if page < 0 else page + by for page in row] for row in step.table]) for by in (0, shift)]
+    error, starts, lengths, positions, rows = dev_ints([0]), dev_ints(step.starts), dev_ints(step.lengths), dev_ints(step.positions), dev_ints(step.rows)
+    out = torch.zeros_like(want)
+    drafts.draft_attention(step.q.to(DEV), far, out, starts, lengths, positions, rows, tables[1], 4, 2, dim, dim ** -0.5, max_nodes=9, max_length=step.max_length,
+                           error_flag=error)
+    assert torch.equal(out, want)
+    parents, tokens = dev_ints([p for t in step.trees for p in t]), dev_ints([3] * 14)
+    for pool, table in ((near, tables[0]), (far, tables[1])):
+        path, counts, following = dev_ints([[0] * 9] * 2), dev_ints([0, 0]), dev_ints([0, 0])
+        moves = cache_moves.PageMoves([pool], 16)
+        drafts.accept_drafts(tokens, parents, tokens, starts, lengths, path, counts, following, moves, table, error)
+        cache_moves.reorder_pages(moves, table, dev_ints([[1, 0]]), dev_ints([0]), dev_ints([33]), 33, error)
+    assert int(counts[0]) > 1 and torch.equal(far[shift:], near) and not torch.equal(near.cpu(), step.pages) and int(error) == 0
+
+
+def test_slots_beyond_32_bits():
+    state = torch.empty((5, 2 ** 30), dtype=torch.uint8, device=DEV)
+    state[3, -64:], state[4, -64:] = 7, 9
+    error = dev_ints([0])
+    cache_moves.reorder_slots(cache_moves.SlotMoves([state]), dev_ints([[3, 4]]), dev_ints([[1, 0]]), error)
+    assert (state[3, -64:] == 9).all() and (state[4, -64:] == 7).all() and int(error) == 0
