@@ -685,3 +685,48 @@ def test_slots_beyond_32_bits():
     error = dev_ints([0])
     cache_moves.reorder_slots(cache_moves.SlotMoves([state]), dev_ints([[3, 4]]), dev_ints([[1, 0]]), error)
     assert (state[3, -64:] == 9).all() and (state[4, -64:] == 7).all() and int(error) == 0
+
+
+def test_calls_at_once_and_graphs_replayed_in_turn():
+    """Two streams with calls of their own, and two captured graphs: nothing of one call is another's."""
+    rng = random.Random(12)
+    steps = [Step(BF16, 12, 2, 128, 16, [900, 77], [random_tree(rng, 20), random_tree(rng, 31)], 5), Step(F32, 6, 2, 32, 16, [800, 500], [random_tree(rng, 9), random_tree(rng, 4)], 6)]
+    calls = []
+    for step in steps:
+        step.check(step.run())
+        q, pages, starts, lengths, positions, rows, table = (step.q.to(DEV), step.pages.to(DEV), dev_ints(step.starts), dev_ints(step.lengths), dev_ints(step.positions),
+                                                             dev_ints(step.rows), dev_ints(step.table))
+        logits, scores = torch.randn(8, 40000, device=DEV), -torch.rand(2, 4, device=DEV)
+        out, best = torch.zeros_like(q), [torch.zeros(2, 8, dtype=t, device=DEV) for t in (F32, torch.int32, torch.int32)]
+
+        def call(step=step, q=q, pages=pages, starts=starts, lengths=lengths, positions=positions, rows=rows, table=table, logits=logits, scores=scores, out=out, best=best):
+            drafts.draft_attention(q, pages, out, starts, lengths, positions, rows, table, step.heads, step.kv_heads, step.dim, step.dim ** -0.5,
+                                   max_nodes=step.max_nodes, max_length=step.max_length)
+            beams.beam_select(logits, scores, *best)
+        call()
+        calls.append((call, [out, *best], [x.clone() for x in (out, *best)]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(20):
+        for (call, outputs, _), stream in zip(calls, streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                for x in outputs:
+                    x.zero_()
+                call()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for _, outputs, wants in calls for a, b in zip(outputs, wants))
+    graphs = []
+    for call, outputs, _ in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        graphs.append(graph)
+    for turn in range(6):
+        for (call, outputs, wants), graph, stream in zip(calls, graphs, streams):
+            with torch.cuda.stream(stream if turn % 2 else torch.cuda.current_stream()):
+                for x in outputs:
+                    x.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for _, outputs, wants in calls for a, b in zip(outputs, wants))
