@@ -141,6 +141,10 @@ def beam_search(engine: Engine, prompt: Sequence[int], num_beams: int, max_new_t
     prompt = [int(t) for t in prompt]
     if not prompt:
         raise ValueError("beam search wants a prompt of at least one token")
+    if not all(0 <= t < vocab for t in prompt):
+        raise ValueError("prompt token is outside the vocabulary")
+    if len(prompt) + max_new_tokens > engine.model.spec.max_position:
+        raise ValueError("prompt plus generated tokens exceeds model context")
     if max_new_tokens == 0:
         return [([], 0.0)]
     search, B = next(_searches), num_beams

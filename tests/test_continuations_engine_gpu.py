@@ -255,3 +255,14 @@ def test_a_search_beside_requests_that_the_scheduler_holds(folders, steps):
         llm.step()
     llm.engine.cache.check()
     assert [list(llm.poll(name).generated) for name in names] == want
+
+
+def test_beam_search_refuses_what_generation_refuses(folders):
+    llm = LLM(folders["a"], dtype="float32", page_size=8, max_tokens=1024)
+    with pytest.raises(ValueError, match="vocabulary"):
+        llm.beam_search([1, 256], 2, 2)
+    with pytest.raises(ValueError, match="context"):
+        llm.beam_search([1] * 500, 2, 13)
+    got = llm.beam_search([1] * 500, 2, 12)                # as far as the model goes
+    assert all(len(t) == 12 for t, _ in got)
+    llm.engine.cache.check()
