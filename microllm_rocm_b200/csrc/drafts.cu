@@ -421,7 +421,7 @@ MLB_EXPORT int mlb_draft_attention(const void* q, const void* pages, void* out, 
     if (words <= 0 || words > MAX_WORDS || max_nodes <= 0 || max_nodes > words * 32)
         return fail(MLB_UNSUPPORTED_SIZE, "draft_attention: %d nodes in masks of %d words (at most %d)", max_nodes, words, MAX_WORDS);
     if (num_pages <= 0 || page_size <= 0 || max_blocks <= 0 || tokens < 0 || sequences < 0 || window < 0) return fail(MLB_INVALID_ARGUMENT, "draft_attention: bad sizes");
-    if (share <= 0 || share % KEYS != 0 || shares <= 0 || (shares > 1 && !scratch)) return fail(MLB_INVALID_ARGUMENT, "draft_attention: bad shares");
+    if (share <= 0 || share % KEYS != 0 || shares <= 0 || (shares > 1 && !scratch) || ((uintptr_t)scratch & 7)) return fail(MLB_INVALID_ARGUMENT, "draft_attention: bad shares");
     const int group = heads / kv_heads, row_tiles = (max_nodes * group + ROWS - 1) / ROWS;
     if (sequences > 65535 || row_tiles * kv_heads > 65535) return fail(MLB_UNSUPPORTED_SIZE, "draft_attention: too many sequences or rows");
     if (tokens == 0 || sequences == 0) return MLB_OK;

@@ -105,7 +105,12 @@ def _ctas(heads: int, row_tiles: int, key_tiles: int, sms: int) -> int:
 
 
 def _memory(alloc, q: torch.Tensor, nbytes: int) -> torch.Tensor:
-    return ops.scratch(nbytes, q, "draft_attention") if alloc is None else alloc(nbytes)
+    if alloc is None:
+        return ops.scratch(nbytes, q, "draft_attention")
+    got = alloc(nbytes)
+    if got.get_device() != q.get_device() or not got.is_contiguous() or got.numel() * got.element_size() < nbytes or got.data_ptr() % 16:
+        raise KernelError(f"draft_attention: `alloc` gave no {nbytes} bytes of the call's device that begin at a multiple of 16")
+    return got
 
 
 def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, starts: torch.Tensor, lengths: torch.Tensor, positions: torch.Tensor,

@@ -164,3 +164,12 @@ def test_plain_definitions():
     assert plain.accept([5, 6, 6, 8, 9, 8], tree, [6, 8, 8, 1, 2, 3]) == ([0, 1, 3], 1)
     scores, parents, tokens = plain.select(torch.zeros(2, 3), torch.tensor([0.0, 0.0]), 7)
     assert parents == [0, 0, 0, 1, 1, 1, -1] and tokens == [0, 1, 2, 0, 1, 2, -1]
+
+
+def test_memory_of_the_callers_own_is_looked_at():
+    q, room = torch.zeros(4, 8), torch.zeros(256, dtype=torch.uint8)
+    at = -room.data_ptr() % 16
+    assert drafts._memory(lambda n: room[at:at + n], q, 64).numel() == 64
+    for bad in (lambda n: room[at:at + n - 1], lambda n: room[at + 8:at + 8 + n], lambda n: room[at:at + 2 * n:2]):
+        with pytest.raises(KernelError, match="64 bytes"):
+            drafts._memory(bad, q, 64)
