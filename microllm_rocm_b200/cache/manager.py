@@ -60,6 +60,7 @@ class _Request:
     length: int = 0
     tables: Dict[str, List[int]] = field(default_factory=dict)     # group -> physical page per block
     slot: Optional[int] = None
+    writes: int = 0          # steps so far that put rows behind `length`, draft steps among them (whose rows the next such step overwrites)
 
 
 class CacheGroup:
@@ -206,6 +207,10 @@ class CacheManager:
                     table[b] = RELEASED
                     self.pages_released_by_window += 1
                     self.tables_version += 1
+
+    def writing(self, request: Hashable) -> None:
+        """A step is about to put rows behind the request's length: what an earlier step left there is lost."""
+        self.requests[request].writes += 1
 
     def release(self, request: Hashable) -> None:
         r = self.requests.pop(request)

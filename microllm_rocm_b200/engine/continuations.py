@@ -37,7 +37,7 @@ class DraftStep:
     entries: List[DraftEntry]
     logits: torch.Tensor
     ctx: object
-    held: List[object]            # the requests' books
+    held: List[Tuple[object, int]]          # the requests' books, and which of their writing steps this one is
 
 
 @dataclass
@@ -96,15 +96,15 @@ def draft_step(engine: Engine, entries: Sequence[DraftEntry]) -> DraftStep:
     logits = engine.model.forward(ctx, engine.cache_views(ctx))
     engine.steps_run += 1
     engine.tokens_run += T
-    return DraftStep(entries, logits, ctx, [engine.cache.requests[e.request] for e in entries])
+    return DraftStep(entries, logits, ctx, [(book, book.writes) for book in (engine.cache.requests[e.request] for e in entries)])
 
 
 def accept_drafts(engine: Engine, step: DraftStep, choices: torch.Tensor) -> List[Accepted]:
     """Walk each tree of `step` along `choices` ([nodes] int32 on the device: the model's own token behind every node), keep the branch in the
-    cache and commit it.  Nothing else may have run for these requests since the step."""
+    cache and commit it.  Refused when one of the requests has taken another step since, a draft step too: its rows lie where this step's were."""
     ctx, cache = step.ctx, engine.cache
-    for e, n, held in zip(step.entries, ctx.seq_pos0_host, step.held):
-        if cache.requests.get(e.request) is not held or cache.length(e.request) != n:
+    for e, n, (book, writes) in zip(step.entries, ctx.seq_pos0_host, step.held):
+        if cache.requests.get(e.request) is not book or book.length != n or book.writes != writes:
             raise StepError(f"request {e.request!r} went on since its draft step")
     A, most = ctx.num_seqs, ctx.tree[2]
     result = torch.empty(A * (most + 2), dtype=torch.int32, device=engine.device)

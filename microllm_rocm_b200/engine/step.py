@@ -184,6 +184,8 @@ class Engine:
         def d(view):
             return dev[view[0]:view[1]]
 
+        for q in requests:
+            cache.writing(q)
         return StepContext(
             num_tokens=T, num_seqs=A, token_ids=d(s_tok), positions=d(s_pos), token_seq=d(s_seq),
             seq_starts=d(s_starts), seq_pos0=d(s_pos0), seq_lens=d(s_lens),
