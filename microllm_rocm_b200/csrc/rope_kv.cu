@@ -2,7 +2,8 @@
 // projection output.
 //
 //   q' = rotate(q + bq, pos)            -> q_out[T, NH*D]            (fp32 or bf16)
-//   k' = rotate(k + bk, pos), v + bv    -> pages[page, 0|1, kvh, slot, :] through the block table
+//   k' = rotate(k + bk, pos), v + bv    -> pages[page, 0|1, kvh, slot, :] through the block table, at the token's position, or
+//                                          at a place of its own (nodes of a drafted tree lie side by side, their positions repeat)
 //
 // Rotation as the reference computes it (src/ops/ops.cpp:861-879, with bias :913-940, per
 // row positions :1086-1115): for pair i, angle = float(pos) * base^(-2 i / D) in fp32,
@@ -27,7 +28,8 @@ struct RopeKvParams {
     int n_partials;          // the projection may arrive as partial results of a split product,
     long long partial_stride;  // `partial_stride` elements apart: they are added here, in order
     const float* bias;       // [(NH+2NKV)*D] or null
-    const int* positions;    // [T] absolute position of each token
+    const int* positions;    // [T] absolute position of each token: what its angles go by
+    const int* places;       // [T] where its key and value go in its sequence's pages, or null: at its position
     const int* token_seq;    // [T] index of the token's sequence in this batch
     const int* block_table;  // [A, max_blocks] physical page of each logical block, -1 if none
     int max_blocks;
@@ -80,9 +82,8 @@ __global__ void rope_kv_kernel(RopeKvParams p) {
         b += src[(size_t)k * p.partial_stride + e1];
     }
     if (p.bias) { a += p.bias[col + e0]; b += p.bias[col + e1]; }
-    const int pos = p.positions[t];
     if (rotate) {
-        const float angle = (float)pos * p.inv_freq[i];
+        const float angle = (float)p.positions[t] * p.inv_freq[i];
         float s, c;
         sincosf(angle, &s, &c);
         const float ra = a * c - b * s;
@@ -96,9 +97,10 @@ __global__ void rope_kv_kernel(RopeKvParams p) {
         return;
     }
     const int kvh = is_k ? head - p.num_heads : head - p.num_heads - p.num_kv_heads;
-    const int block = pos / p.page_size, slot = pos % p.page_size;
+    const int place = (p.places ? p.places : p.positions)[t];
+    const int block = place / p.page_size, slot = place % p.page_size;
     int page = -1;
-    if (pos >= 0 && block < p.max_blocks) page = p.block_table[(size_t)p.token_seq[t] * p.max_blocks + block];
+    if (place >= 0 && block < p.max_blocks) page = p.block_table[(size_t)p.token_seq[t] * p.max_blocks + block];
     if (page < 0 || page >= p.num_pages) {
         if (p.error_flag) atomicExch(p.error_flag, 1);
         return;                                   // never write outside the pool
@@ -140,22 +142,23 @@ __global__ void rope_kv_split_half_x4_kernel(RopeKvParams p) {
     const size_t col = (size_t)head * p.head_dim;
     float4 ba = make_float4(0.f, 0.f, 0.f, 0.f), bb = ba;
     float sn[4] = {0.f, 0.f, 0.f, 0.f}, cs[4] = {1.f, 1.f, 1.f, 1.f};
-    int pos = 0, page = -1;
+    int place = 0, page = -1;
     if (working) {
         if (p.bias) {
             ba = *reinterpret_cast<const float4*>(p.bias + col + i);
             bb = *reinterpret_cast<const float4*>(p.bias + col + i + half);
         }
-        pos = p.positions[t];
         if (!is_v && !p.cos_sin) {
+            const int pos = p.positions[t];
             const float4 f = *reinterpret_cast<const float4*>(p.inv_freq + i);
             const float fr[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) sincosf((float)pos * fr[k], &sn[k], &cs[k]);
         }
         if (!is_q) {
-            const int block = pos / p.page_size;
-            if (pos >= 0 && block < p.max_blocks) page = p.block_table[(size_t)p.token_seq[t] * p.max_blocks + block];
+            place = (p.places ? p.places : p.positions)[t];
+            const int block = place / p.page_size;
+            if (place >= 0 && block < p.max_blocks) page = p.block_table[(size_t)p.token_seq[t] * p.max_blocks + block];
         }
     }
     pdl_wait();
@@ -194,7 +197,7 @@ __global__ void rope_kv_split_half_x4_kernel(RopeKvParams p) {
         return;
     }
     const int kvh = is_v ? head - p.num_heads - p.num_kv_heads : head - p.num_heads;
-    const int slot = pos % p.page_size;
+    const int slot = place % p.page_size;
     if (page < 0 || page >= p.num_pages) {
         if (p.error_flag) atomicExch(p.error_flag, 1);
         return;
@@ -235,7 +238,7 @@ MLB_EXPORT int mlb_rope_kv_write(const float* qkv, long long ld, int n_partials,
                                  const float* inv_freq, int rot_dim, int interleaved, void* q_out, int q_dtype,
                                  void* pages, int kv_dtype, int num_pages, int page_size, int tokens,
                                  int num_heads, int num_kv_heads, int head_dim, int* error_flag,
-                                 const float* cos_sin, cudaStream_t stream) {
+                                 const float* cos_sin, const int* places, cudaStream_t stream) {
     if (tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || head_dim % 2 != 0)
         return fail(MLB_INVALID_ARGUMENT, "rope_kv_write: bad head sizes");
     if (rot_dim < 0 || rot_dim > head_dim || rot_dim % 2 != 0)
@@ -246,7 +249,7 @@ MLB_EXPORT int mlb_rope_kv_write(const float* qkv, long long ld, int n_partials,
         return fail(MLB_INVALID_ARGUMENT, "rope_kv_write: cache geometry missing");
     if (tokens == 0) return MLB_OK;
     if (n_partials < 1) return fail(MLB_INVALID_ARGUMENT, "rope_kv_write: n_partials must be at least 1");
-    RopeKvParams p{qkv, ld, n_partials, partial_stride, bias, positions, token_seq, block_table, max_blocks, inv_freq, rot_dim, interleaved,
+    RopeKvParams p{qkv, ld, n_partials, partial_stride, bias, positions, places, token_seq, block_table, max_blocks, inv_freq, rot_dim, interleaved,
                    q_out, pages, num_pages, page_size, tokens, num_heads, num_kv_heads, head_dim, error_flag, nullptr};
     const int key = q_dtype * 2 + kv_dtype;
     // the model's own case in 16-byte pieces: split-half over the whole head, eight-element alignment

@@ -86,7 +86,7 @@ _SIGNATURES = {
     "rope_kv.cu": {
         "mlb_rope_kv_write": [c_void_p, c_longlong, c_int, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                               c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_int,
-                              c_int, c_int, c_int, c_void_p, c_void_p, c_void_p],
+                              c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
         "mlb_rope_table": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p],
     },
     "attention_plain.cu": {
@@ -786,12 +786,15 @@ def rope_kv_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], positions: to
                   token_seq: torch.Tensor, block_table: Optional[torch.Tensor], inv_freq: torch.Tensor,
                   rot_dim: int, interleaved: bool, q_out: torch.Tensor, pages: Optional[torch.Tensor],
                   num_heads: int, num_kv_heads: int, head_dim: int, error_flag: Optional[torch.Tensor],
-                  cos_sin: Optional[torch.Tensor] = None) -> None:
+                  cos_sin: Optional[torch.Tensor] = None, places: Optional[torch.Tensor] = None) -> None:
     """Bias, rotation and the K/V store for a fused [T, (NH+2NKV)*D] fp32 projection output
     (or its [S, T, width] partial results, which are summed here).
     `pages` is [num_pages, 2, NKV, page_size, D]; None makes the call query-only.
-    `cos_sin` [T, rot_dim/2, 2] fp32 (from `rope_table`) spares the kernel the sines and cosines."""
+    `cos_sin` [T, rot_dim/2, 2] fp32 (from `rope_table`) spares the kernel the sines and cosines.
+    `places` [T] int32: where the tokens' keys and values go in their sequences' pages; None: at their positions."""
     _need(positions, "positions", torch.int32, 1)
+    if places is not None:
+        _need(places, "places", torch.int32, 1)
     n_partials, partial_stride = 1, 0
     if qkv.dim() == 3:
         _need(qkv, "qkv", torch.float32, 3)
@@ -802,7 +805,7 @@ def rope_kv_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], positions: to
     _need(q_out, "q_out", dims=2)
     T = qkv.shape[0]
     width = (num_heads + 2 * num_kv_heads) * head_dim
-    if qkv.shape[1] != width or q_out.shape != (T, num_heads * head_dim) or positions.shape[0] != T:
+    if qkv.shape[1] != width or q_out.shape != (T, num_heads * head_dim) or positions.shape[0] != T or (places is not None and places.shape[0] != T):
         raise KernelError("rope_kv_write: shapes do not agree")
     if inv_freq.shape[0] * 2 != rot_dim:
         raise KernelError("rope_kv_write: inv_freq must have rot_dim/2 entries")
@@ -825,7 +828,7 @@ def rope_kv_write(qkv: torch.Tensor, bias: Optional[torch.Tensor], positions: to
         qkv.data_ptr(), width, n_partials, partial_stride, _ptr(bias), positions.data_ptr(), token_seq.data_ptr(), _ptr(block_table), max_blocks,
         inv_freq.data_ptr(), rot_dim, 1 if interleaved else 0, q_out.data_ptr(), dtype_tag(q_out),
         _ptr(pages), dtype_tag(pages) if pages is not None else F32, num_pages, page_size, T,
-        num_heads, num_kv_heads, head_dim, _ptr(error_flag), _ptr(cos_sin), _stream()))
+        num_heads, num_kv_heads, head_dim, _ptr(error_flag), _ptr(cos_sin), _ptr(places), _stream()))
 
 
 def rope_table(positions: torch.Tensor, inv_freq: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:

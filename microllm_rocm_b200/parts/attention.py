@@ -42,6 +42,7 @@ def distance_rows(buckets: int, far: float):
 @register_mixer("attention")
 class Attention(Mixer):
     graph_safe = True
+    takes_drafts = True
 
     def __init__(self, params: dict, rt: Runtime, position: Optional[PositionEncoding] = None):
         self.prefix = params.get("prefix", "")
@@ -63,8 +64,6 @@ class Attention(Mixer):
         if self.rotary is None:        # no rotation: an empty table makes the kernel pass q/k through
             self._no_rot = torch.zeros(0, dtype=torch.float32, device=rt.device)
         self.w_qkv = self.b_qkv = self.w_o = self.b_o = None
-        # a drafted tree's tokens are rotated by one number and stored by another: where the rotation takes the step's table of angles
-        self.takes_drafts = self.rotary is None or (self.rotary.rotary_dim == self.d and not self.rotary.interleaved and self.d % 16 == 0)
 
     # --- declarations -----------------------------------------------------------------
     def cache_need(self):
@@ -156,8 +155,8 @@ class Attention(Mixer):
                 if cos_sin is None:
                     table = ctx.buffer("attention.rope_table", (T, rot // 2, 2), torch.float32)
                     cos_sin = ctx.step_values[key] = ops.rope_table(ctx.positions, inv_freq, out=table)
-            ops.rope_kv_write(qkv, self.b_qkv, ctx.positions if ctx.tree is None else ctx.places, ctx.token_seq, cache.block_table, inv_freq, rot, inter,
-                              q, pages, self.nh, self.nkv, self.d, ctx.error_flag, cos_sin)
+            ops.rope_kv_write(qkv, self.b_qkv, ctx.positions, ctx.token_seq, cache.block_table, inv_freq, rot, inter,
+                              q, pages, self.nh, self.nkv, self.d, ctx.error_flag, cos_sin, ctx.places)
         o = ctx.buffer("attention.o", (T, self.nh * self.d), self.rt.dtype)
         if ctx.tree is not None:
             from ..kernels import drafts

@@ -1,11 +1,15 @@
 """Drafted trees and beams at their edges."""
+import dataclasses
+import random
+
 import pytest
 import torch
 
 from microllm_rocm_b200.engine import DraftEntry, OutOfPages, StepEntry, StepError
 from microllm_rocm_b200.engine.loading import load_engine
 from microllm_rocm_b200.kernels import ops
-from tests.helpers import make_folder
+from tests.helpers import FP32_ATOL, make_folder, random_tokens, tiny_config
+from tests.test_continuations_gpu import DEV, dev_ints, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +63,66 @@ def test_a_step_that_did_not_run_overtakes_nothing(folders):
     accepted, = engine.accept_drafts(step, argmax(step.logits))
     assert accepted.nodes[0] == 0 and engine.cache.length("r") == 3 + len(accepted.nodes)
     assert len(engine.accept_drafts(other, argmax(other.logits))) == 1
+
+
+# ------------------------------------------------------------------------------ memory that is not aligned
+@pytest.mark.parametrize("what", ["bias", "angles", "both"])
+def test_trees_are_rotated_by_depth_wherever_the_weights_lie(folders, what):
+    """A bias and frequencies that begin 4 bytes off the 16 that wide loads want: the positions of a tree's nodes are still their depths."""
+    prompt, vocab = random_tokens(20, 384, 1), tiny_config("b").vocab_size
+    rng = random.Random(4)
+    entry = DraftEntry("r", [rng.randrange(vocab) for _ in range(12)], random_tree(rng, 12))
+    found = []
+    for moved in (False, True):
+        engine = load_engine(folders["b"], dtype="float32", page_size=16, max_tokens=256)
+        for block in engine.model.blocks if moved else ():
+            mixer = block.mixer
+
+            def off(t):
+                room = torch.empty(t.numel() + 4, dtype=t.dtype, device=t.device)
+                at = (20 - room.data_ptr() % 16) // 4 % 4
+                room[at:at + t.numel()] = t
+                assert room[at:].data_ptr() % 16 == 4
+                return room[at:at + t.numel()]
+            if what != "angles":
+                assert mixer.b_qkv is not None
+                mixer.b_qkv = off(mixer.b_qkv)
+            if what != "bias":
+                mixer.rotary = dataclasses.replace(mixer.rotary, inv_freq=off(mixer.rotary.inv_freq))
+        assert engine.cache.add("r")
+        engine.step([StepEntry("r", prompt)])
+        step = engine.draft_step([entry])
+        found.append(step.logits.float().cpu())
+        engine.check_device_errors()
+    assert float((found[0] - found[1]).abs().max()) <= 2 * FP32_ATOL
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d, rot, interleaved, table, off", [(64, 64, False, True, 0), (64, 64, False, False, 0), (64, 64, False, True, 1), (64, 64, True, False, 0), (64, 32, False, False, 0),
+                                                             (40, 40, False, True, 0), (6, 6, False, False, 0), (32, 0, False, False, 0)])
+def test_tokens_are_rotated_by_position_and_stored_by_place(dtype, d, rot, interleaved, table, off):
+    """Every token alone, at its position, has the bits that all of them together have at their places."""
+    nh, nkv, page, T = 4, 2, 8, 21
+    rng = random.Random(d + rot)
+    g = torch.Generator().manual_seed(d)
+    width = (nh + 2 * nkv) * d
+    qkv = torch.randn(T, width, generator=g).to(DEV)
+    bias = torch.randn(width + off, generator=g).to(DEV)[off:]
+    freq = torch.rand(rot // 2, generator=g).to(DEV)
+    positions = [rng.randrange(40) for _ in range(T)]      # they repeat
+    places = rng.sample(range(40), T)
+    blocks, error = dev_ints([[3, 0, 4, 1, 2]]), dev_ints([0])
+
+    def write(rows, where, at):
+        q, pages = torch.full((len(rows), nh * d), 7.0, dtype=dtype, device=DEV), torch.full((5, 2, nkv, page, d), 7.0, dtype=dtype, device=DEV)
+        ops.rope_kv_write(qkv[rows].contiguous(), bias, dev_ints(where), dev_ints([0] * len(rows)), blocks, freq, rot, interleaved, q, pages, nh, nkv, d, error,
+                          ops.rope_table(dev_ints(where), freq) if table else None, at)
+        return q, pages[blocks[0].long()].permute(0, 3, 1, 2, 4).reshape(40, 2 * nkv * d)
+    q, rows = write(list(range(T)), positions, dev_ints(places))
+    for t in range(T):
+        alone, kept = write([t], [positions[t]], None)
+        assert torch.equal(q[t], alone[0]) and torch.equal(rows[places[t]], kept[positions[t]])
+    nobodys = [i for i in range(40) if i not in places]
+    assert (rows[nobodys] == 7.0).all() and int(error) == 0
+    write([0], [0], dev_ints([40]))                        # a place that no block holds
+    assert int(error) == 1
