@@ -18,8 +18,9 @@
 //                 are issued behind the product that reads P, so "scores are there" also says that the accumulator is (the tensor pipe runs in order)
 //     warps 4-11  softmax of stream (warp - 4) / 4: mask in the tiles that need one, running maximum and sum in fp32 with base-2
 //                 exponentials, the accumulator rescaled only when a row's maximum has grown by 2^8
-// In tiles that not every row sees alike the value rows are looked through: one that holds a number which is not finite is cleared for the product (0 * NaN
-// would reach rows that do not see it) and the rows that do see it become NaN; value rows that nobody sees are cleared too.
+// In tiles that not every row sees alike the value rows are looked through: a number that is not finite is cleared for the product (0 * NaN would reach rows
+// that do not see it), and the rows that do see it add it, in its column, where their results go out (this way out costs calls without such values 1 %: 16 ragged sequences
+// 77.0 -> 77.9 us for two layers, 4 of 8,192 keys 157.4 -> 158.9); value rows that nobody sees are cleared as a whole.
 //
 // What bounds it.  Long calls: the products and the softmax beside one another (40 heads of 8, 50 nodes, 4 sequences, for every 16,384 keys of them all: products alone 55 us,
 // softmax alone 61, both 70; memory alone 40).  4 sequences of 8,192 keys and 64 nodes take 70 us a layer with the join: 43 GFLOP, 0.62 PFLOP/s, of rows that fill 320 of
@@ -76,6 +77,7 @@ constexpr int CHUNK = 32;                    // scores that a softmax thread has
 
 struct TcParams {
     __nv_bfloat16* out;             // [T, NH * D]
+    const __nv_bfloat16* pages;     // [num_pages, 2, NKV, page_size, D]: what the key and value map describes
     const int* starts;              // [A + 1]
     const int* lengths;             // [A]
     const int* positions;           // [T]
@@ -423,6 +425,7 @@ struct Shared {
     Sequence s;
     unsigned odd[3][2][4];               // [streams, or both][turn & 1]: which of a tile's value rows are not finite
     float2 norm[2 * BM];                 // the rows' maxima and sums, for streams that share the rows
+    bool reads_odd[2 * BM];              // and whether they see such a value row
 };
 static_assert(sizeof(Shared) <= SHARED_BYTES, "what the warps tell one another");
 
@@ -682,42 +685,39 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             const int pos = p.positions[s.token0 + node];
             const int lo_r = p.window > 0 ? max(0, pos - p.window + 1) : 0;
             float m_used = -INFINITY, l = 0.0f;
-            bool sees_odd = false;
+            bool odd_score = false, odd_value = false;        // the row sees a score that is NaN or +inf, a value in an edge tile that is not finite
             // A tile that not every row sees alike holds a node, or a cached key in front of some node's window.  The latest position is at
             // most length + n - 1.
             const int window_end = p.window > 0 ? max(0, total - p.window) : 0;
+            auto is_edge = [&](int kbase) { return kbase + BN > s.length || kbase < window_end; };
+            auto seen_of = [&](int from) {                    // which of the 32 keys from `from` on the thread's row sees
+                unsigned bits = bit_range(lo_r - from, s.length - from);             // cached keys
+                const int j = from - s.length;                // the node at the first of them, if any
+                if (j + 31 >= 0 && j < s.n) {
+                    // the 32 mask bits from bit j on (j may be negative)
+                    const int* const row = p.masks + (size_t)(s.token0 + node) * p.words;
+                    const int at = j >> 5;                    // rounds down
+                    const unsigned low = at >= 0 && at < p.words ? (unsigned)row[at] : 0u, high = at + 1 >= 0 && at + 1 < p.words ? (unsigned)row[at + 1] : 0u;
+                    unsigned nodes = __funnelshift_r(low, high, (unsigned)(j & 31)) & bit_range(-j, s.n - j);
+                    if (p.window > 0 && lo_r > s.length) {
+                        // a window shorter than the tree is deep
+                        for (unsigned left = nodes; left; left &= left - 1) {
+                            const int b = __ffs(left) - 1;
+                            if (p.positions[s.token0 + j + b] < lo_r) nodes &= ~(1u << b);
+                        }
+                    }
+                    bits |= nodes;
+                }
+                return bits;
+            };
             bool first = true;
             for (int t = paired ? 0 : stream; t < n_tiles; t += dt, ++turn, first = false) {
                 const int kbase = (s.first + walk.tile + t) * BN;
-                const bool edge = kbase + BN > s.length || kbase < window_end;
+                const bool edge = is_edge(kbase);
                 unsigned seen[4];
                 if (edge) {
 #pragma unroll 1
-                    for (int w = 0; w < 4; ++w) seen[w] = 0u;
-                    if (mine) {
-                        const int j0 = kbase - s.length;  // the node at column 0, if any
-                        const int* const row = p.masks + (size_t)(s.token0 + node) * p.words;
-#pragma unroll 1
-                        for (int w = 0; w < 4; ++w) {
-                            const int from = kbase + w * 32, j = j0 + w * 32;
-                            unsigned bits = bit_range(lo_r - from, s.length - from);             // cached keys
-                            if (j + 31 >= 0 && j < s.n) {
-                                // the 32 mask bits from bit j on (j may be negative)
-                                const int at = j >> 5;    // rounds down
-                                const unsigned low = at >= 0 && at < p.words ? (unsigned)row[at] : 0u, high = at + 1 >= 0 && at + 1 < p.words ? (unsigned)row[at + 1] : 0u;
-                                unsigned nodes = __funnelshift_r(low, high, (unsigned)(j & 31)) & bit_range(-j, s.n - j);
-                                if (p.window > 0 && lo_r > s.length) {
-                                    // a window shorter than the tree is deep
-                                    for (unsigned left = nodes; left; left &= left - 1) {
-                                        const int b = __ffs(left) - 1;
-                                        if (p.positions[s.token0 + j + b] < lo_r) nodes &= ~(1u << b);
-                                    }
-                                }
-                                bits |= nodes;
-                            }
-                            seen[w] = bits;
-                        }
-                    }
+                    for (int w = 0; w < 4; ++w) seen[w] = mine ? seen_of(kbase + w * 32) : 0u;
                 }
                 lag_point();
                 ok = wait_all(&sh.s_full[stream], turn & 1, 49);
@@ -746,7 +746,7 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                     }
                     if (edge) tmem_wait_st();
                     // a score that is NaN or +inf: the row becomes NaN (fmaxf passes over a NaN)
-                    if (!(top < INFINITY)) { sees_odd = true; top = -INFINITY; }
+                    if (!(top < INFINITY)) { odd_score = true; top = -INFINITY; }
                     const float m_new = fmaxf(m_used, top * p.scale_log2);
                     const bool grow = m_new > m_used + RESCALE_STEP;      // also true for the first finite maximum
                     const float alpha = grow ? (m_used == -INFINITY ? 0.0f : fast_exp2(m_used - m_new)) : 1.0f;
@@ -799,10 +799,19 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                         }
                         const unsigned mark = __ballot_sync(0xffffffffu, odd);
                         if (lane == 0) sh.odd[which][buffer][quarter] = mark;
-                        if (odd || nobodys) {
+                        if (nobodys) {
 #pragma unroll 1
                             for (int i = 0; i < SPANS * 8; ++i)
                                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(vrow + (i / 8) * (BN * ROW_BYTES) + ((i ^ lane) & 7) * 16), "r"(0u) : "memory");
+                        } else if (odd) {
+#pragma unroll 1
+                            for (int i = 0; i < SPANS * 32; ++i) {
+                                const uint32_t at = vrow + (i / 32) * (BN * ROW_BYTES) + (i % 32) * 4;
+                                uint32_t v;
+                                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
+                                v &= ((v & 0x7f80u) == 0x7f80u ? 0u : 0xffffu) | ((v >> 16 & 0x7f80u) == 0x7f80u ? 0u : 0xffff0000u);
+                                asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+                            }
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // for the tensor core
                     }
@@ -811,7 +820,7 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                     ok = wait_all(&sh.v_checked[which], buffer, 51);
                     if (!ok) break;
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) sees_odd |= (seen[w] & *(volatile unsigned*)&sh.odd[which][buffer][w]) != 0u;
+                    for (int w = 0; w < 4; ++w) odd_value |= (seen[w] & *(volatile unsigned*)&sh.odd[which][buffer][w]) != 0u;
                     ++looked[paired];
                 }
                 tc_fence_before();
@@ -821,10 +830,11 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             if (!ok) break;
             item0 += 2 * n_tiles;
             // ---- the rows' results.  Streams that share the rows meet: each takes half of the columns of both accumulators.
-            float weight[2] = {0.0f, 0.0f}, m_all = m_used, l_all = sees_odd ? NAN : l;
+            float weight[2] = {0.0f, 0.0f}, m_all = m_used, l_all = odd_score ? NAN : l;
             weight[stream] = 1.0f;
             if (!paired) {
                 sh.norm[stream * BM + r] = make_float2(m_used, l_all);
+                sh.reads_odd[stream * BM + r] = odd_value;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(smem_u32(&sh.norms_there));
                 ok = wait_all(&sh.norms_there, shared_pieces & 1, 52);
@@ -835,6 +845,7 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                 weight[1] = b.x == -INFINITY ? 0.0f : fast_exp2(b.x - m_all);
                 l_all = a.y * weight[0] + b.y * weight[1];
                 if (isnan(a.y) || isnan(b.y)) l_all = NAN;
+                odd_value = sh.reads_odd[r] || sh.reads_odd[BM + r];
             }
             // whose accumulators this warp reads, and which there are
             const bool made[2] = {true, paired || n_tiles > 1}, has[2] = {!paired || stream == 0, paired ? stream == 1 : n_tiles > 1};
@@ -879,6 +890,29 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
                     __syncwarp();
                 }
                 if (mine && !whole && (paired || stream == 0)) p.part_norm[part * BM + r] = make_float2(m_all, l_all);
+                if (odd_value && l_all != 0.0f) {
+                    // the values that were cleared, once more from the pages: whatever its weight, one that is not finite makes its column so
+                    const int* const table = p.table + (size_t)walk.a * p.max_blocks;
+#pragma unroll 1
+                    for (int w = 0; w < 4 * n_tiles; ++w) {
+                        const int from = (s.first + walk.tile) * BN + w * 32;
+                        if (!is_edge(from / BN * BN)) continue;
+#pragma unroll 1
+                        for (unsigned left = seen_of(from); left; left &= left - 1) {
+                            const int key = from + __ffs(left) - 1, page = table[key / p.page_size];
+                            if (page < 0 || page >= p.num_pages) continue;
+                            const __nv_bfloat16* const v = p.pages + ((((size_t)page * 2 + 1) * p.kv_heads + kvh) * p.page_size + key % p.page_size) * D;
+#pragma unroll 1
+                            for (int col = c_begin * 16; col < c_end * 16; ++col) {
+                                const float x = __bfloat162float(v[col]);
+                                if (fabsf(x) < INFINITY) continue;
+                                if (whole) p.out[row * D + col] = __float2bfloat16(__bfloat162float(p.out[row * D + col]) + x);
+                                else p.part_out[(part * D + col) * BM + r] += x;
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
             }
             tc_fence_before();                            // the accumulators were read before what the next piece's first P releases
             if (!paired) {
@@ -1057,7 +1091,7 @@ MLB_EXPORT int mlb_draft_attention_tc(const void* q, const void* pages, void* ou
         const int status = encode(&map_kv, pages, 2, dims, strides, box);
         if (status != MLB_OK) return status;
     }
-    TcParams p{(__nv_bfloat16*)out, starts, lengths, positions, masks, table, words, max_blocks, num_pages, page_size, BN / page_size, heads, kv_heads, group,
+    TcParams p{(__nv_bfloat16*)out, (const __nv_bfloat16*)pages, starts, lengths, positions, masks, table, words, max_blocks, num_pages, page_size, BN / page_size, heads, kv_heads, group,
                tile_nodes, (max_nodes + tile_nodes - 1) / tile_nodes, window, max_nodes, stretch, ctas, sequences, tokens,
                (int)std::min((long long)max_blocks * page_size, 1ll << 30), scale * LOG2E, nullptr, nullptr, nullptr, error_flag};
     if (ctas > 1) {

@@ -118,7 +118,9 @@ def draft_attention(q: torch.Tensor, pages: torch.Tensor, out: torch.Tensor, sta
                     window: Optional[int] = None, *, max_nodes: int, max_length: int, error_flag: Optional[torch.Tensor] = None,
                     alloc: Optional[Callable[[int], torch.Tensor]] = None) -> None:
     """out[t, h] = softmax(scale q[t, h] . k) v over what node t sees: its sequence's cached tokens and the nodes of its mask, of both only
-    those of the last `window` positions where one is given.  A node that sees nothing gets zeros.
+    those of the last `window` positions where one is given.  A node that sees nothing gets zeros.  A key that scores NaN or +inf makes its row NaN, one that
+    scores -inf weighs nothing; a value that is not finite makes its column inf or NaN, as the sum has it, in the rows that see its key with a weight above zero
+    (in fp32), and no other.
 
     `q` and `out` [T, heads * D], `pages` [pages, 2, kv heads, page, D] of the same type (fp32 or bf16); `positions` and `masks` as `draft_masks`
     makes them (any other mask over a sequence's nodes will do); `block_table` [sequences, blocks] int32.

@@ -1,5 +1,6 @@
-"""Drafted trees and beams at their edges."""
+"""Drafted trees and beams at their edges.  Attention is held against 64 bits with the bounds of test_continuations_gpu.py (Step.check)."""
 import dataclasses
+import math
 import random
 
 import pytest
@@ -9,7 +10,7 @@ from microllm_rocm_b200.engine import DraftEntry, OutOfPages, StepEntry, StepErr
 from microllm_rocm_b200.engine.loading import load_engine
 from microllm_rocm_b200.kernels import ops
 from tests.helpers import FP32_ATOL, make_folder, random_tokens, tiny_config
-from tests.test_continuations_gpu import DEV, dev_ints, random_tree
+from tests.test_continuations_gpu import BF16, DEV, F32, Step, dev_ints, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -126,3 +127,72 @@ def test_tokens_are_rotated_by_position_and_stored_by_place(dtype, d, rot, inter
     assert (rows[nobodys] == 7.0).all() and int(error) == 0
     write([0], [0], dev_ints([40]))                        # a place that no block holds
     assert int(error) == 1
+
+
+# ------------------------------------------------------------------------------ values that are not finite
+SPOILED = [
+    # dtype, heads, kv heads, dim, lengths, nodes, window
+    (F32, 4, 2, 32, [300, 200], [6, 3], None),
+    (F32, 4, 2, 200, [300, 200], [6, 3], 60),
+    (BF16, 4, 2, 128, [300, 20], [6, 3], None),            # one row tile, whose two streams share the rows
+    (BF16, 4, 2, 64, [90, 20], [6, 3], 60),                # the same with one key tile
+    (BF16, 12, 2, 64, [300, 200], [40, 50], 100),          # a row tile a stream
+    (BF16, 12, 2, 128, [5000, 3000], [50, 3], None),       # items that lie in several CTAs
+    (BF16, 28, 4, 128, [5000, 3000, 40], [60, 3, 64], 700),
+]
+
+
+def poison(step, seq, place, column, value, kv_head=1, which=1):
+    step.pages[step.table[seq][place // 16], which, kv_head, place % 16, column] = value
+
+
+@pytest.mark.parametrize("case", range(len(SPOILED)))
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+def test_a_value_that_is_not_finite_stays_in_its_column(case, value):
+    """Of a cached key in a tile that all rows see alike, of the last cached one, of one at a window's start, and of nodes; one column each of one kv head, and
+    one column where +inf and -inf meet.  The row that 64 bits say, in every column and head."""
+    dtype, heads, kv_heads, dim, lengths, nodes, window = SPOILED[case]
+    rng = random.Random(case)
+    step = Step(dtype, heads, kv_heads, dim, 16, lengths, [random_tree(rng, n) for n in nodes], case, window)
+    clean = step.pages.clone()
+    n = lengths[0]
+    for column, place in enumerate((5, n // 2, n - 1, max(0, n - (window or n) + 2), n, n + 2)):
+        poison(step, 0, place, 3 * column, value)
+    poison(step, 0, n - 2, 20, math.inf)
+    poison(step, 0, n + 1, 20, -math.inf)
+    poison(step, 1, lengths[1] + 1, 21, value)
+    want = step.want()
+    got = step.run()
+    there = torch.isfinite(want)
+    assert 0 < int((~there).sum()) < want.numel() / 2
+    seen = got.cpu().double().view(want.shape)
+    assert torch.equal(torch.isfinite(seen), there)
+    assert torch.equal(seen[~there].nan_to_num(5.0, 6.0, 7.0), want[~there].nan_to_num(5.0, 6.0, 7.0))
+    step.pages = clean                                     # (the bound goes by the sizes of the finite values)
+    step.check(torch.where(there, seen, 0.0).view(got.shape), torch.where(there, want, 0.0))
+
+
+@pytest.mark.parametrize("case", range(len(SPOILED)))
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_a_node_of_one_kv_head_that_is_not_finite_reaches_every_head_of_its_group(case, value):
+    """Its key (queries of mixed sign make every score NaN) and its value, in all columns: every element of the rows below it in that group's heads, and no other."""
+    dtype, heads, kv_heads, dim, lengths, nodes, window = SPOILED[case]
+    rng = random.Random(case)
+    step = Step(dtype, heads, kv_heads, dim, 16, lengths, [random_tree(rng, n) for n in nodes], case, window)
+    want = step.want()
+    clean = step.pages.clone()
+    below = torch.zeros(want.shape, dtype=torch.bool)
+    group = heads // kv_heads
+    for t in range(nodes[0]):
+        if (step.rows[t][0] >> 2) & 1:
+            below[t, group:2 * group] = True
+    assert 0 < int(below.any(-1).any(-1).sum()) < nodes[0]
+    for which in (0, 1, None):
+        step.pages = clean.clone()
+        for half in (0, 1) if which is None else (which,):
+            poison(step, 0, lengths[0] + 2, slice(None), value, which=half)
+        got = step.run()
+        seen = got.cpu().double().view(want.shape)
+        assert torch.equal(~torch.isfinite(seen), below), which
+        step.pages = clean
+        step.check(torch.where(below, 0.0, seen).view(got.shape), torch.where(below, 0.0, want))
