@@ -8,9 +8,9 @@ import torch
 
 from microllm_rocm_b200.engine import DraftEntry, OutOfPages, StepEntry, StepError
 from microllm_rocm_b200.engine.loading import load_engine
-from microllm_rocm_b200.kernels import ops
+from microllm_rocm_b200.kernels import beams, ops
 from tests.helpers import FP32_ATOL, make_folder, random_tokens, tiny_config
-from tests.test_continuations_gpu import BF16, DEV, F32, Step, dev_ints, random_tree
+from tests.test_continuations_gpu import BF16, DEV, F32, Step, check_select, dev_ints, random_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -196,3 +196,44 @@ def test_a_node_of_one_kv_head_that_is_not_finite_reaches_every_head_of_its_grou
         assert torch.equal(~torch.isfinite(seen), below), which
         step.pages = clean
         step.check(torch.where(below, 0.0, seen).view(got.shape), torch.where(below, 0.0, want))
+
+
+# ------------------------------------------------------------------------------ equal scores of different beams
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("far", [-80.0, -33.25, -20.5])
+def test_equal_scores_of_different_beams_go_to_the_lower_one(far, dtype):
+    """A beam whose score is `far` and that has one continuation, beside one whose second continuation lies that far below its first: 64 bits say equal or nearly so, and
+    a distance that was scaled by a rounded constant would put the higher beam first."""
+    V = 9000
+    logits = torch.full((2, V), -math.inf, dtype=dtype, device=DEV)
+    logits[0, 7] = 3.0
+    logits[1, 11], logits[1, 12] = 0.0, far
+    check_select(logits, torch.tensor([[far, 0.0]], device=DEV), 3)
+    flipped, scores = logits.flip(0).contiguous(), torch.tensor([[0.0, far]], device=DEV)
+    if far == -20.5 and dtype == BF16:
+        # One thread has both terms: 1 + e^-20.5 = 1 + 1.25e-9 is 1 in fp32, whose half step is 2^-25 = 3.0e-8 below and 6.0e-8 above 1, so a normaliser of 0 where 64 bits
+        # have 1.25e-9.  The candidates 1.25e-9 apart are equal then, and the lower beam's comes first.
+        got = torch.zeros(1, 3, device=DEV), dev_ints([[0] * 3]), dev_ints([[0] * 3])
+        beams.beam_select(flipped, scores, *got)
+        assert got[1].tolist() == [[0, 0, 1]] and got[2].tolist() == [[11, 12, 7]] and got[0].tolist() == [[0.0, far, far]]
+    else:
+        check_select(flipped, scores, 3)
+    logits[1, 11], logits[1, 12] = 1000.0, 1000.0 + far if dtype == F32 else 920.0
+    check_select(logits, torch.tensor([[far if dtype == F32 else -80.0, 0.0]], device=DEV), 3)
+
+
+def test_scores_are_the_logarithms_of_the_softmax_nearly_in_64_bits():
+    """Scores that come out near 0, where fp32 shows what the normaliser is worth.  A term of the row's sum, 2^-a of the largest, is off by 2^-22 of the function (its
+    documented error) and by its argument's rounding, (a + 1) 2^-24 log 2 at most.  Weighted by its share of the sum these are 2^-22 and 2^-24 times the entropy and one (12 at
+    most for 50,000 tokens), log2 e's rounding is 2^-26 of the entropy, and sums of 32 terms add 5 x 2^-24: 2^-24 (4 + 13 + 3 + 5) = 1.5e-6, if all went one way."""
+    g = torch.Generator().manual_seed(3)
+    for scale, V in ((0.1, 50000), (1.0, 9000), (2.5, 50000), (6.0, 50000)):
+        rows = torch.randn(8, V, generator=g) * scale
+        top = rows.max(1).values.double()
+        start = (torch.logsumexp(rows.double(), 1) - top).float()              # the best continuation comes out within 1e-6 of 0
+        out = (torch.zeros(8, 1, device=DEV), torch.zeros(8, 1, dtype=torch.int32, device=DEV), torch.zeros(8, 1, dtype=torch.int32, device=DEV))
+        beams.beam_select(rows.to(DEV), start.view(8, 1).to(DEV), *out)
+        want = start.double() + top - torch.logsumexp(rows.double(), 1)
+        off = (out[0].cpu().double().view(8) - want).abs().max()
+        print(f"scale {scale}, {V} tokens: off by {float(off):.2e}")
+        assert float(off) <= 1.5e-6
