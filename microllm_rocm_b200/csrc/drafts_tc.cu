@@ -30,7 +30,7 @@
 // Tried and slower: tiles of 64 keys with two score buffers a stream (Q's rows come from shared memory as often for half the keys), two softmax threads a row (159 us against
 // 145 for two layers of the long call above), an issuing warp for each stream (92 us a layer against 70: the streams' products alternate in the tensor pipe).
 //
-// Every wait on an mbarrier is bounded; when a bound is hit the error flag is raised, the CTA waits (bounded) for the copies in flight, frees
+// Every wait on an mbarrier is bounded; when a bound is hit the error flag is raised, the CTA waits (bounded) for the products and copies in flight, frees
 // its tensor memory and returns.
 #include "common.cuh"
 #include "packed.cuh"
@@ -68,7 +68,11 @@ static_assert(128 * FEW_REGISTERS + 256 * MANY_REGISTERS <= THREADS * 168, "no m
 constexpr int STREAM_COLS = 256;             // tensor memory of a stream: scores (then P as bf16 pairs) [0, 128), accumulator [128, 128 + D)
 constexpr int TMEM_COLS = 2 * STREAM_COLS;
 constexpr int O_COL = BN;
-constexpr int SPIN_LIMIT = 1 << 21;          // polls of up to 2 us each
+#ifndef MLB_SPIN_LIMIT                       // (the tests build objects whose waits run out at once)
+#define MLB_SPIN_LIMIT (1 << 21)
+#endif
+constexpr int SPIN_LIMIT = MLB_SPIN_LIMIT;   // polls of up to 2 us each
+constexpr int DRAIN_LIMIT = 1 << 14;         // the same for what is in flight when a wait has run out: microseconds, or never
 constexpr int MAX_PAGES_PER_TILE = 16;
 constexpr int MAX_WORDS = 8;
 constexpr float LOG2E = 1.4426950408889634f;
@@ -119,6 +123,10 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* er
         if (mbar_try_wait(bar, parity)) return true;
     if (error_flag) atomicCAS(error_flag, 0, code);          // the first failure is the one worth reporting
     return false;
+}
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < DRAIN_LIMIT; ++i)
+        if (mbar_try_wait(bar, parity)) return;
 }
 // true in exactly one lane of the (converged) warp
 __device__ __forceinline__ bool elect_one() {
@@ -419,7 +427,7 @@ struct Walk {
 };
 
 struct Shared {
-    unsigned long long q_full, q_empty, slot_full[SLOTS], slot_empty[SLOTS], s_full[2], p_full[2], o_full[2], v_checked[3], norms_there, o_read;
+    unsigned long long q_full, q_empty, slot_full[SLOTS], slot_empty[SLOTS], s_full[2], p_full[2], o_full[2], v_checked[3], norms_there, o_read, stopped;
     uint32_t tmem_base;
     int failed, unit, end, a, base, stretch, lead, pieces, issued;      // pieces, issued: whose copies were asked for
     Sequence s;
@@ -455,7 +463,8 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
         mbar_init(smem_u32(&sh.v_checked[2]), 8);
         mbar_init(smem_u32(&sh.norms_there), 8);
         mbar_init(smem_u32(&sh.o_read), 8);
-        sh.failed = (base & 1023u) ? 1 : 0;                 // the swizzle pattern wants 1024-byte alignment
+        mbar_init(smem_u32(&sh.stopped), 1);                // all products that were issued are done
+        sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -496,13 +505,14 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
     const uint32_t tmem_base = sh.tmem_base;
     const int stretch = sh.stretch, lead = sh.lead;
     Walk walk;
-    walk.unit = sh.failed ? sh.end : sh.unit;
+    const bool misplaced = (base & 1023u) != 0;             // the swizzle pattern wants 1024-byte alignment
+    walk.unit = misplaced ? sh.end : sh.unit;
     walk.end = sh.end;
     walk.a = sh.a;
     walk.base = sh.base;
     walk.known = sh.a;
     walk.s = sh.s;
-    if (sh.failed && threadIdx.x == 0 && p.error_flag) atomicCAS(p.error_flag, 0, 40);
+    if (misplaced && threadIdx.x == 0 && p.error_flag) atomicCAS(p.error_flag, 0, 40);
 
     // Ring items in order of need, piece after piece.  Shared key tiles: K0 K1 V0 K2 V1 K3 ..; a row tile a stream: K0 V0 K1 V1 ..: K(0 .. dt - 1)
     // first, then for every t: V(t), K(t + dt).  A piece of n key tiles is 2 n items.
@@ -562,6 +572,7 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
             bool ok = true;
             int pieces = 0;
             for (; walk.next(p, stretch, lead); ++pieces) {
+                lag_point();
                 if (pieces > 0) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&sh.q_empty), (pieces - 1) & 1, p.error_flag, 41)) != 0;
                 if (!ok) break;
                 if (lane == 0) {
@@ -928,10 +939,18 @@ draft_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __gri
 
     tc_fence_before();
     __syncthreads();
-    if (sh.failed && warp == 0 && lane == 0) {
-        // give the copies in flight a bounded chance to land before the CTA's memory goes away
-        if (sh.pieces > 0) mbar_wait(smem_u32(&sh.q_full), (sh.pieces - 1) & 1, nullptr, 0);
-        for (int i = max(0, sh.issued - SLOTS); i < sh.issued; ++i) mbar_wait(smem_u32(&sh.slot_full[i % SLOTS]), (i / SLOTS) & 1, nullptr, 0);
+    if (sh.failed) {
+        // What is in flight gets a bounded chance to end before the CTA's memory goes away: copies write shared memory, products read it and write tensor
+        // memory.  (A CTA that did not fail has waited for all of them.)
+        if (warp == 0 && lane == 0) {
+            if (sh.pieces > 0) mbar_drain(smem_u32(&sh.q_full), (sh.pieces - 1) & 1);
+            for (int i = max(0, sh.issued - SLOTS); i < sh.issued; ++i) mbar_drain(smem_u32(&sh.slot_full[i % SLOTS]), (i / SLOTS) & 1);
+        } else if (warp == 1) {
+            if (elect_one()) umma_commit(smem_u32(&sh.stopped));
+            __syncwarp();
+            mbar_drain(smem_u32(&sh.stopped), 0);
+        }
+        __syncwarp();
     }
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)TMEM_COLS) : "memory");

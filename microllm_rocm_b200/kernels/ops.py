@@ -157,8 +157,10 @@ def lagged_latent_sources():
 
 
 def lagged_draft_sources():
-    """And of the attention of drafted trees: both copying and issuing warps, and a softmax warp of each stream."""
-    return [("drafts_tc.cu", {"HEAD_DIM": 128, "MLB_LAG_WARP": w}) for w in (0, 1, 5, 10)]
+    """And of the attention of drafted trees: both copying and issuing warps, and a softmax warp of each stream; then those whose waits run out after so
+    many polls."""
+    return ([("drafts_tc.cu", {"HEAD_DIM": 128, "MLB_LAG_WARP": w}) for w in (0, 1, 5, 10, 3)] + [("drafts_tc.cu", {"HEAD_DIM": 64, "MLB_LAG_WARP": w}) for w in (1, 3)] +
+            [("drafts_tc.cu", {"HEAD_DIM": 128, "MLB_SPIN_LIMIT": n}) for n in (0, 1, 4)])
 
 
 _PACKED_FORMATS = {c_void_p: "P", c_int: "i", c_longlong: "q", c_float: "f"}

@@ -237,3 +237,45 @@ def test_scores_are_the_logarithms_of_the_softmax_nearly_in_64_bits():
         off = (out[0].cpu().double().view(8) - want).abs().max()
         print(f"scale {scale}, {V} tokens: off by {float(off):.2e}")
         assert float(off) <= 1.5e-6
+
+
+# ------------------------------------------------------------------------------ warps that are late, waits that run out
+def cut_steps(dim):
+    """Streams that share the rows, a row tile a stream, and CTAs that walk through many items, whose queries follow one another into the same place."""
+    rng = random.Random(9)
+    sizes = [1 + rng.randrange(40) for _ in range(70)]
+    return [Step(BF16, 6, 1, dim, 16, [900, 64], [random_tree(rng, 20), random_tree(rng, 3)], 1), Step(BF16, 6, 1, dim, 16, [700, 130], [random_tree(rng, 40), random_tree(rng, 64)], 2, 60),
+            Step(BF16, 6, 6, dim, 16, [rng.randrange(300) for _ in sizes], [random_tree(rng, n) for n in sizes], 3)]
+
+
+def with_defines(monkeypatch, defines):
+    monkeypatch.setitem(ops.TEST_DEFINES, "drafts_tc.cu", {k: v for k, v in defines.items() if k != "HEAD_DIM"})
+
+
+@pytest.mark.parametrize("which", [i for i, (_, d) in enumerate(ops.lagged_draft_sources()) if "MLB_LAG_WARP" in d])
+def test_items_that_follow_one_another_do_not_depend_on_which_warp_is_late(which, monkeypatch):
+    _, defines = ops.lagged_draft_sources()[which]
+    steps = cut_steps(defines["HEAD_DIM"])
+    want = [s.run() for s in steps]
+    for s, w in zip(steps, want):
+        s.check(w)
+    with_defines(monkeypatch, defines)
+    for s, w in zip(steps, want):
+        assert torch.equal(s.run(), w) and int(s.error) == 0
+
+
+@pytest.mark.parametrize("polls", [0, 1, 4])
+def test_a_wait_that_runs_out_is_reported_and_leaves_nothing_behind(polls, monkeypatch):
+    """Every wait gives up after a few polls: the error flag says so (or, where none ran out, the rows are right), the kernel ends, and the next launch is as ever."""
+    steps = cut_steps(128)
+    want = [s.run() for s in steps]
+    with_defines(monkeypatch, {"MLB_SPIN_LIMIT": polls})
+    for s, w in zip(steps, want):
+        for _ in range(3):
+            got = s.run()
+            code = int(s.error)
+            assert 40 <= code <= 54 if polls == 0 else code == 0 or 40 <= code <= 54
+            assert code != 0 or torch.equal(got, w)
+    monkeypatch.undo()
+    for s, w in zip(steps, want):
+        assert torch.equal(s.run(), w) and int(s.error) == 0
