@@ -44,7 +44,7 @@ def require_gpu(device: Optional[str] = None) -> torch.device:
 
 def prepare_kernels(model=None) -> None:
     """Compile, at once and in parallel, every kernel object this model will ask for."""
-    sources = ops.base_sources()
+    sources = ops.base_sources() + ops.search_sources()
     if model is not None:
         for part in model.parts():
             for item in part.kernel_sources():

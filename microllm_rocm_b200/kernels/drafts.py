@@ -47,8 +47,10 @@ def _sm_count(device_index: int) -> int:
     return got
 
 
-def tc_sources(head_dim: int):
-    return [("drafts_tc.cu", {"HEAD_DIM": head_dim})] if head_dim in TC_HEAD_DIMS else []
+def sources(head_dim: int, fp32: bool):
+    """(source, defines) of what steps with drafted trees launch for layers of this head size."""
+    tc = [("drafts_tc.cu", {"HEAD_DIM": head_dim})] if head_dim in TC_HEAD_DIMS and not fp32 else []
+    return [("drafts.cu", {}), ("cache_moves.cu", {})] + tc
 
 
 def tc_supported(head_dim: int, page_size: int, group: int, scale: float) -> bool:

@@ -225,9 +225,14 @@ def part_sources():
             ("linear_attention.cu", {}), ("post_norm.cu", {}), ("streams.cu", {})]
 
 
+def search_sources():
+    """(source, defines) of beam search's own kernels, which any model may ask for."""
+    return [("beams.cu", {}), ("cache_moves.cu", {})]
+
+
 def continuation_sources():
     """(source, defines) of the kernels for several continuations of a request: drafted trees and beams."""
-    return [("drafts.cu", {}), ("drafts_tc.cu", {"HEAD_DIM": 64}), ("drafts_tc.cu", {"HEAD_DIM": 128}), ("beams.cu", {}), ("cache_moves.cu", {})]
+    return [("drafts.cu", {}), ("drafts_tc.cu", {"HEAD_DIM": 64}), ("drafts_tc.cu", {"HEAD_DIM": 128})] + search_sources()
 
 
 def all_sources():

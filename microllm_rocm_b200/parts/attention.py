@@ -18,7 +18,7 @@ from typing import Dict, Optional
 import torch
 
 from ..kernels import attention as attention_kernels
-from ..kernels import gemm_bf16, ops
+from ..kernels import drafts, gemm_bf16, ops
 from ..kernels.linear import linear
 from .base import Mixer, PagedKVNeed, PagedKVView, PositionEncoding, Runtime, StepContext, WeightSpec, register_mixer
 
@@ -102,10 +102,11 @@ class Attention(Mixer):
         self.b_o = tensors.get("o_proj.bias")
 
     def kernel_sources(self):
+        own = drafts.sources(self.d, self.rt.is_fp32)
         if self.rt.is_fp32:
-            return []
+            return own
         return (gemm_bf16.sources(engine_only=True) + attention_kernels.mma_sources(self.d)
-                + attention_kernels.tc_sources(self.d))
+                + attention_kernels.tc_sources(self.d) + own)
 
     def replay_key(self):
         if self.out_bias:
@@ -159,7 +160,6 @@ class Attention(Mixer):
                               q, pages, self.nh, self.nkv, self.d, ctx.error_flag, cos_sin, ctx.places)
         o = ctx.buffer("attention.o", (T, self.nh * self.d), self.rt.dtype)
         if ctx.tree is not None:
-            from ..kernels import drafts
             masks, _, most = ctx.tree
             drafts.draft_attention(q, cache.pages, o, ctx.seq_starts, ctx.seq_pos0, ctx.positions, masks, cache.block_table, self.nh, self.nkv, self.d,
                                    self.scale, self.window, max_nodes=most, max_length=ctx.max_seq_len, error_flag=ctx.error_flag,
