@@ -398,8 +398,6 @@ MLB_EXPORT int mlb_accept_drafts(const void* const* bases, int count, long long 
     return check_launch("accept_drafts");
 }
 
-MLB_EXPORT int mlb_moves_max_storages() { return MAX_STORAGES; }
-
 MLB_PACKED(mlb_reorder_slots)
 MLB_PACKED(mlb_reorder_pages)
 MLB_PACKED(mlb_accept_drafts)

@@ -109,8 +109,7 @@ def accept_drafts(engine: Engine, step: DraftStep, choices: torch.Tensor) -> Lis
     A, most = ctx.num_seqs, ctx.tree[2]
     result = torch.empty(A * (most + 2), dtype=torch.int32, device=engine.device)
     path, counts, following = result[:A * most].view(A, most), result[A * most:A * most + A], result[A * most + A:]
-    groups = list(cache.groups)
-    for i, group in enumerate(groups):
+    for group in cache.groups:
         drafts.accept_drafts(ctx.token_ids, ctx.tree[1], choices, ctx.seq_starts, ctx.seq_pos0, path, counts, following, cache.page_moves(group),
                              ctx.block_tables[group], engine.error_flag)
     host = result.tolist()
@@ -205,7 +204,7 @@ def _search(engine, names, prompt, max_new_tokens, end_token, device, vocab):
         if any(v != v for v in values):
             raise StepError("a beam's logits are not finite")
         tokens = [tokens[p] + ([] if ended[p] else [t]) if p >= 0 else None for p, t in zip(parents, picks)]
-        was_ended, ended = ended, [p < 0 or (end_token is not None and t == end_token) for p, t in zip(parents, picks)]
+        ended = [p < 0 or (end_token is not None and t == end_token) for p, t in zip(parents, picks)]
         scores = out_scores
         if all(ended) or max(len(t) for t in tokens if t is not None) >= max_new_tokens:
             return [(t, v) for t, v in zip(tokens, values) if t is not None]
