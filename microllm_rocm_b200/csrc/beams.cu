@@ -11,7 +11,8 @@
 //
 // The `wanted` largest of a set, without sorting it: every warp gives the four largest of its lanes' own maxima, and the wanted-th largest of these 32 elements (all of
 // them different ones) bounds what is chosen: no chosen element lies below it, and the few at or above it are ranked by counting.  (Above 32 wanted: the least of the warps'
-// eighth largest.)  So many equal elements that they do not fit the list are chosen one after the other.
+// eighth largest.)  So many equal elements that they do not fit the list are chosen one after the other (8 rows of 152,064 logits, all but 100 masked by a finite value: 64 us
+// instead of 13; by -inf, which is never chosen: 13).
 #include <cfloat>
 
 #include "common.cuh"
@@ -503,6 +504,7 @@ long long aligned(long long bytes) { return (bytes + 15) / 16 * 16; }
 
 template <typename T>
 void launch_slices(const SelectParams& p, int rows, cudaStream_t stream) {
+    // (160 rows of 50,256 fp32, bf16 logits in pieces 19.1, 18.0 us; of 50,257 element by element 17.8, 19.1; 8 rows 10.7, 10.4 and 10.5, 11.3)
     const bool wide = ((uintptr_t)p.logits & 15) == 0 && p.ld * sizeof(T) % 16 == 0;
     if (wide) launch_kernel(select_slices_kernel<T, true>, dim3(p.parts, rows), THREADS, SLICE * sizeof(T), stream, p);
     else launch_kernel(select_slices_kernel<T, false>, dim3(p.parts, rows), THREADS, 0, stream, p);

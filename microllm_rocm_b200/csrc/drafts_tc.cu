@@ -1,5 +1,6 @@
 // Attention of drafted trees over the paged bf16 cache on the fifth-generation tensor cores, heads of 64 or 128 (-DHEAD_DIM).  What a
-// row sees is csrc/drafts.cu's; P is rounded to bf16 for the second product.
+// row sees is csrc/drafts.cu's.  P is rounded to bf16 for the second product, which tensor cores take no wider beside bf16 values: half a step of each weight, both ways
+// (outputs are off by 0.0019 to 0.0023 of their norm against 64 bits, of which 0.0017 is the output's own rounding).  The row's sum is of the weights before that.
 //
 // An item is the rows (node, head of the group) of up to 2 x floor(128 / group) nodes of one sequence and kv head.  It has two streams of work, each
 // with four softmax warps (a thread a row), its own scores and its own accumulator in tensor memory:
@@ -23,7 +24,7 @@
 // 77.0 -> 77.9 us for two layers, 4 of 8,192 keys 157.4 -> 158.9); value rows that nobody sees are cleared as a whole.
 //
 // What bounds it.  Long calls: the products and the softmax beside one another (40 heads of 8, 50 nodes, 4 sequences, for every 16,384 keys of them all: products alone 55 us,
-// softmax alone 61, both 70; memory alone 40).  4 sequences of 8,192 keys and 64 nodes take 70 us a layer with the join: 43 GFLOP, 0.62 PFLOP/s, of rows that fill 320 of
+// softmax alone 61, both 70; memory alone 40).  4 sequences of 8,192 keys and 64 nodes take 70 us a layer with the join (73 to 75 in a long series of calls): 43 GFLOP, 0.62 PFLOP/s, of rows that fill 320 of
 // 384 tensor-core rows.  Short calls: a chain that nothing fills, from the wait for the kernel in front on: cutting the line 1.4 us, block table, copies and first scores 2.5,
 // a turn 1.6, results 2.3, then the join 5 (one sequence of 2,074 keys and 26 nodes, 12 heads of 2: 14.8 us).
 //

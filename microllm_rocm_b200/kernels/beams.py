@@ -12,7 +12,7 @@ from .cache_moves import INT, _address, need_current, need_on
 
 MAX_BEAMS = 32              # csrc/beams.cu
 MAX_WANTED = 64
-SLICE = 8192                # logits a CTA takes
+SLICE = 8192                # csrc/beams.cu: logits of a slice (a CTA takes one or more of a row)
 
 ops.register_signatures("beams.cu", {
     "mlb_beam_select": [c_void_p, c_int, c_longlong, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p,
